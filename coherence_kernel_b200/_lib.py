@@ -31,6 +31,13 @@ class DecodeConfig(ctypes.Structure):
     _fields_ = [("hidden", _u32), ("max_tokens", _u32), ("eps", _f), ("moe", MoeConfig)]
 
 
+class KvConfig(ctypes.Structure):
+    """ck_kv_config (include/ck_b200.h)."""
+    _fields_ = [("n_kv_heads", _u32), ("head_dim", _u32), ("block_tokens", _u32), ("n_blocks", _u32),
+                ("cache_type", _u32), ("reserved", _u32), ("block_stride", _u64), ("token_stride", _u64),
+                ("head_stride", _u64)]
+
+
 # name -> (restype, argtypes); every symbol include/*.h declares
 SIGNATURES = {
     "ck_last_error": (ctypes.c_char_p, []),
@@ -104,6 +111,12 @@ SIGNATURES = {
     "ck_decode_step_replay": (_i32, [_p, _p]),
     "ck_decode_step_status": (_i32, [_p, _u32, _p]),
     "ck_decode_step_destroy": (None, [_p]),
+    "ck_rmsnorm_add": (_i32, [_i32, _p, _u64, _i32, _p, _p, _u64, _p, _i32, _p, _u64, _u32, _u32, _f, _p]),
+    "ck_kv_plan": (_i32, [_p, _p, _u32, _p, _u64, _u32, _p, _p, _u32, _u32, _u32, _p, _p, _p, _p, _p, _p, _p]),
+    "ck_kv_append": (_i32, [ctypes.POINTER(KvConfig), _i32, _p, _u64, _p, _u64, _p, _u32, _p, _p, _p]),
+    "ck_paged_attention_workspace_bytes": (_sz, [_u32, _u32, _u32]),
+    "ck_paged_attention": (_i32, [ctypes.POINTER(KvConfig), _u32, _i32, _p, _u64, _p, _p, _p, _u64, _u32, _p, _p,
+                                  _u32, _u32, _f, _i32, _u32, _p, _u64, _p, _p, _sz, _p]),
     # the handle door
     "fk_metal_pipeline_external": (_ll, [ctypes.c_char_p, _ll, ctypes.c_char_p, _ll]),
     "fk_metal_buf_alloc_external": (_ll, [_ll]),

@@ -541,6 +541,122 @@ int ck_moe_layer_bf16(const ck_moe_config *c, const void *x, uint32_t ntok, cons
                           s);
 }
 
+// ------------------------------------------------------------------------------ paged KV cache
+int ck_rmsnorm_add(int x_type, const void *x, uint64_t x_stride, int res_type, const void *res, void *res_out,
+                   uint64_t res_stride, const float *gain, int out_type, void *out, uint64_t out_stride, uint32_t ntok,
+                   uint32_t hidden, float eps, void *s) {
+    return fail(ck::launch_rmsnorm_add(x_type, x, x_stride, res_type, res, res_out, res_stride, gain, out_type, out,
+                                       out_stride, ntok, hidden, eps, S(s)),
+                "ck_rmsnorm_add");
+}
+
+int ck_kv_plan(const int32_t *len_in, const int32_t *new_tokens, uint32_t nreq, int32_t *table, uint64_t table_stride,
+               uint32_t max_blocks, int32_t *free_blocks, const int32_t *count_in, uint32_t n_blocks,
+               uint32_t block_tokens, uint32_t ntok, int32_t *len_out, int32_t *count_out, int32_t *kv_len,
+               int32_t *q_start, int64_t *slots, int32_t *positions, void *s) {
+    if (nreq > ck::KV_PLAN_MAX_REQUESTS || ntok >= 1u << 30 || block_tokens == 0 || max_blocks == 0 || n_blocks == 0 ||
+        (uint64_t)max_blocks * block_tokens >= 1u << 30 || (uint64_t)n_blocks * block_tokens >= 1u << 31)
+        return fail(CK_ESHAPE, "ck_kv_plan");
+    if (!count_in || !count_out || !q_start || !free_blocks || (ntok && (!slots || !positions)) ||
+        (nreq && (!len_in || !new_tokens || !table || !len_out || !kv_len)) || table_stride < max_blocks)
+        return fail(CK_EARG, "ck_kv_plan");
+    const ck::KvPlanParams p = {len_in, new_tokens, count_in, table, free_blocks, len_out, count_out, kv_len, q_start,
+                                positions, slots, table_stride, nreq, ntok, max_blocks, n_blocks,
+                                ck::FastDiv::make(block_tokens)};
+    return fail(ck::launch_kv_plan(p, S(s)), "ck_kv_plan");
+}
+
+namespace {
+int check_kv(const ck_kv_config *c) {
+    if (!c) return CK_EARG;
+    if (c->n_kv_heads == 0 || c->head_dim == 0 || c->head_dim % 8 || c->head_dim > 256 || c->block_tokens == 0 ||
+        c->n_blocks == 0 || (uint64_t)c->n_blocks * c->block_tokens >= 1u << 31)
+        return CK_ESHAPE;
+    if (c->cache_type != CK_BF16 && c->cache_type != CK_F16) return CK_EARG;
+    if (c->block_stride % 8 || c->token_stride % 8 || c->head_stride % 8) return CK_EARG;
+    return 0;
+}
+inline bool off16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+}  // namespace
+
+int ck_kv_append(const ck_kv_config *c, int in_type, const void *k, uint64_t k_stride, const void *v, uint64_t v_stride,
+                 const int64_t *slots, uint32_t ntok, void *k_cache, void *v_cache, void *s) {
+    int rc = check_kv(c);
+    if (rc) return fail(rc, "ck_kv_append config");
+    if (in_type != CK_F32 && in_type != CK_F16 && in_type != CK_BF16) return fail(CK_EARG, "ck_kv_append type");
+    if (ntok == 0) return 0;
+    const uint64_t row = (uint64_t)c->n_kv_heads * c->head_dim;
+    if (row > 1u << 30 || ntok * row >= 1ull << 32) return fail(CK_ESHAPE, "ck_kv_append");
+    if (!k || !v || !slots || !k_cache || !v_cache || off16(k) || off16(v) || off16(k_cache) || off16(v_cache))
+        return fail(CK_EARG, "ck_kv_append");
+    if (k_stride < row || v_stride < row || k_stride % 8 || v_stride % 8) return fail(CK_EARG, "ck_kv_append strides");
+    const ck::KvAppendParams p = {k, v, k_stride, v_stride, slots, k_cache, v_cache, c->block_stride, c->token_stride,
+                                  c->head_stride, (int64_t)c->n_blocks * c->block_tokens, ntok, (int)c->cache_type,
+                                  ck::FastDiv::make(c->block_tokens), ck::FastDiv::make((uint32_t)(row / 8)),
+                                  ck::FastDiv::make(c->head_dim / 8)};
+    return fail(ck::launch_kv_append(p, in_type, S(s)), "ck_kv_append");
+}
+
+size_t ck_paged_attention_workspace_bytes(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim) {
+    if (n_heads == 0 || n_kv_heads == 0 || n_heads % n_kv_heads || head_dim == 0 || head_dim % 8 || head_dim > 256)
+        return 0;
+    return al(ck::attn_few_workspace_bytes(head_dim));
+}
+
+int ck_paged_attention(const ck_kv_config *c, uint32_t n_heads, int io_type, const void *q, uint64_t q_stride,
+                       const void *k_cache, const void *v_cache, const int32_t *table, uint64_t table_stride,
+                       uint32_t max_blocks, const int32_t *kv_len, const int32_t *q_start, uint32_t nreq, uint32_t ntok,
+                       float scale, int causal, uint32_t window, void *out, uint64_t out_stride, float *lse, void *ws,
+                       size_t wsb, void *s) {
+    int rc = check_kv(c);
+    if (rc) return fail(rc, "ck_paged_attention config");
+    const uint64_t row = (uint64_t)n_heads * c->head_dim;
+    if (n_heads == 0 || n_heads % c->n_kv_heads || (uint64_t)ntok * n_heads >= 1u << 30 || max_blocks == 0 ||
+        (uint64_t)max_blocks * c->block_tokens >= 1u << 30 || nreq >= 1u << 30)
+        return fail(CK_ESHAPE, "ck_paged_attention");
+    if (io_type != CK_F32 && io_type != (int)c->cache_type) return fail(CK_EARG, "ck_paged_attention type");
+    if (nreq == 0 || ntok == 0) return 0;
+    if (!q || !out || !k_cache || !v_cache || !table || !kv_len || !q_start || !ws || off16(q) || off16(out) ||
+        off16(k_cache) || off16(v_cache) || off16(ws))
+        return fail(CK_EARG, "ck_paged_attention");
+    if (q_stride < row || out_stride < row || q_stride % 8 || out_stride % 8 || table_stride < max_blocks)
+        return fail(CK_EARG, "ck_paged_attention strides");
+    if (wsb < ck_paged_attention_workspace_bytes(n_heads, c->n_kv_heads, c->head_dim))
+        return fail(CK_EARG, "ck_paged_attention workspace");
+    ck::AttnParams p = {};
+    p.q = q;
+    p.k = k_cache;
+    p.v = v_cache;
+    p.out = out;
+    p.lse = lse;
+    p.table = table;
+    p.kv_len = kv_len;
+    p.q_start = q_start;
+    p.part_o = (float *)ws;
+    p.q_stride = q_stride;
+    p.out_stride = out_stride;
+    p.table_stride = table_stride;
+    p.block_stride = c->block_stride;
+    p.token_stride = c->token_stride;
+    p.head_stride = c->head_stride;
+    p.nreq = nreq;
+    p.ntok = ntok;
+    p.n_kv = c->n_kv_heads;
+    p.head_dim = c->head_dim;
+    p.max_blocks = max_blocks;
+    p.n_blocks = c->n_blocks;
+    p.btd = ck::FastDiv::make(c->block_tokens);
+    p.gd = ck::FastDiv::make(n_heads / c->n_kv_heads);
+    p.row_split = 0x7fffffffu;
+    p.scale_log2 = scale * 1.44269504088896341f;
+    // a window as long as the table row bounds nothing
+    p.window = window >= (uint64_t)max_blocks * c->block_tokens ? 0 : (int)window;
+    p.causal = causal;
+    p.io_type = io_type;
+    p.cache_type = (int)c->cache_type;
+    return fail(ck::launch_attn_few(p, S(s)), "ck_paged_attention");
+}
+
 // Reads the device error word of a layer's workspace (synchronizes the stream).
 int ck_moe_layer_status(const ck_moe_config *c, uint32_t ntok, const void *ws, void *s) {
     if (check_cfg(c) || !ws) return fail(CK_EARG, "ck_moe_layer_status");

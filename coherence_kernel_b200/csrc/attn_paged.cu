@@ -1,0 +1,508 @@
+// attn_paged.cu -- attention of few new tokens per request over a paged K/V cache (decode steps,
+// short drafts, and every form the chunk kernel does not take), and the joining of partial results.
+//
+//   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale q_i . k_j - m_i),  j over the visible keys
+//
+// in one pass over the keys with the running maximum and sum of each row.  The rows of a tile are 16
+// (token, grouped query head) pairs that share a K/V head, so each K and V row is read once for all
+// of them.  HBM bounds it: a decode step does 4 x rows flop per cache element.
+//
+// A CTA has four warps.  A unit is 64 keys; each warp takes 16 of them and has a ring of its own of
+// STAGES x (16 K rows + 16 V rows) in shared memory, filled by 16-byte asynchronous copies whose
+// page lookups run a unit ahead, so no warp waits for another until the item's end.  Ring and cursor run
+// on across items.  S = Q K^T and O += P V run on mma.m16n8k16 (the 16 rows are one tile: the
+// fifth-generation instructions start at 64), with fp32 accumulation; P goes from the first product's
+// registers to the second's operands.
+//
+// With f32 queries and outputs the operands keep fp32's accuracy: Q and P are split into TERMS terms
+// of the cache's type, each the rounding of the remainder (bf16: three of 8 bits; f16: two of 11, Q's rows
+// scaled to [1, 2) by a power of two first), and every product with a K or V element is exact in the
+// accumulator.  (A remainder may be zero or negative, so infinities of V are kept out of every such product and
+// added afterwards.)  With 2-byte queries P is rounded once to the cache's type, an error of half an ulp of each
+// weight, below the output's own rounding.
+#include "attn_sched.cuh"
+
+#include <type_traits>
+
+namespace ck {
+namespace attn {
+namespace {
+
+constexpr int TR = 16, KC = 64, WARPS = 4, WK = KC / WARPS;  // rows, keys per unit, warps, keys per warp
+using S = Sched<TR, KC, false>;
+
+template <int DP, int TERMS>
+struct Few {
+    static constexpr int ROW = DP * 2;  // bytes of a K or V row in shared memory
+    static constexpr int STAGES = DP <= 64 ? 4 : 3;
+    static constexpr int STAGE = 2 * WK * ROW;
+    static constexpr int RING = WARPS * STAGES * STAGE;
+    // the query tile (all terms), and after the last key the 16 x DP fp32 sum over the warps
+    static constexpr int QO = (TERMS * ROW > DP * 4 ? TERMS * ROW : DP * 4) * TR;
+    static constexpr int SMEM = RING + QO;
+    static constexpr int CTAS = DP <= 64 ? 3 : DP <= 128 ? 2 : 1;  // per SM
+};
+
+CK_DEV void cp16(uint32_t dst, const void *src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+CK_DEV void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+CK_DEV void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+CK_DEV void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+CK_DEV void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+template <int TYPE>
+CK_DEV void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (TYPE == T_BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// the pair (lo, hi) rounded to the type, and the remainders left in lo, hi
+template <int TYPE>
+CK_DEV uint32_t split2(float &lo, float &hi) {
+    const uint32_t w = pack2(TYPE, lo, hi);
+    if constexpr (TYPE == T_BF16) {
+        lo -= __uint_as_float(w << 16);
+        hi -= __uint_as_float(w & 0xFFFF0000u);
+    } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+        lo -= f.x;
+        hi -= f.y;
+    }
+    return w;
+}
+// a pair of V elements with its infinities and NaNs replaced by zero
+template <int TYPE>
+CK_DEV uint32_t finite2(uint32_t w, bool &bad) {
+    constexpr uint32_t M = TYPE == T_BF16 ? 0x7F80u : 0x7C00u;
+    const bool l = (w & M) == M, h = (w >> 16 & M) == M;
+    bad |= l | h;
+    return (l ? 0u : w & 0xFFFFu) | (h ? 0u : w & 0xFFFF0000u);
+}
+
+template <int TYPE, int DP, int TERMS>
+__global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(const AttnParams p) {
+    using F = Few<DP, TERMS>;
+    constexpr int ROW = F::ROW, NS = F::STAGES, PIECES = DP / 8, COPIES = WK * PIECES / 32;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ typename S::Shared sh;
+    __shared__ float row_scale[TR], wm[WARPS][TR], wl[WARPS][TR];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t ring = smem_u32(smem) + warp * NS * F::STAGE, qs = smem_u32(smem) + F::RING;
+    float *osum = reinterpret_cast<float *>(smem + F::RING);
+    grid_dep_trigger_small();
+    grid_dep_wait();
+
+    long long U;
+    int C;
+    Pos pos;
+    Geo geo;
+    if (!S::find(p, sh, (int)gridDim.x, (int)blockIdx.x, U, C, pos, geo)) return;
+    const int n = (int)(S::start(U, C, blockIdx.x + 1) - S::start(U, C, blockIdx.x));
+    typename S::Cursor use, fill;
+    use.set(p, pos, geo);
+    fill = use;
+
+    // lane l < 16 looks up key l of the warp's next 16: its element offset, or -1 to fill with zeros
+    // (past the tile's last key, so that what the page holds there never meets a product)
+    const auto lookup = [&]() -> int64_t {
+        const int j = fill.g.lo + fill.at.c * KC + warp * WK + (lane & 15);
+        if (j >= fill.g.hi) return -1;
+        const int64_t at = key_offset(p, fill.at.r, j);
+        return at < 0 ? -1 : at + (int64_t)(fill.at.h * p.head_stride);
+    };
+    const auto copy_in = [&](int stage, int64_t off) {
+        const uint32_t base = ring + stage * F::STAGE;
+#pragma unroll
+        for (int i = 0; i < COPIES; ++i) {
+            const int idx = i * 32 + lane, row = idx / PIECES, c = idx % PIECES;
+            const int64_t at = __shfl_sync(0xffffffffu, off, row);
+            const bool live = at >= 0 && c * 8 < (int)p.head_dim;
+            const int64_t e = live ? at + c * 8 : 0;
+            const uint32_t dst = base + row * ROW + ((c ^ (row & 7)) << 4);
+            cp16(dst, static_cast<const uint16_t *>(p.k) + e, live);
+            cp16(dst + WK * ROW, static_cast<const uint16_t *>(p.v) + e, live);
+        }
+    };
+    int filled = 0;
+    int64_t off = lookup();
+    const auto fill_next = [&]() {
+        if (filled < n) {
+            copy_in(filled % NS, off);
+            if (++filled < n) {
+                fill.next(p);
+                off = lookup();
+            }
+        }
+        cp_commit();  // an empty group past the end keeps the count of groups in step
+    };
+    for (int i = 0; i < NS - 1; ++i) fill_next();
+
+    float o[DP / 8][4];
+    float m[2], l[2];
+    int row_lo[2], row_hi[2];
+    int all_lo = 0, all_hi = 0;  // keys that every row of the tile sees
+    bool bad = false;
+    bool fresh = true;
+    int first_c = 0, segment = 0;
+    for (int i = 0; i < n; ++i) {
+        const int rows = use.q.nq * (int)p.gd.d, row0 = use.at.t * TR;
+        if (fresh) {
+            fresh = false;
+            first_c = use.at.c;
+            bad = false;
+#pragma unroll
+            for (int d = 0; d < DP / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.0f;
+            // the query tile: eight threads per row
+            const int r = threadIdx.x >> 3, part = threadIdx.x & 7, row = row0 + r;
+            const bool live = row < rows;
+            const uint32_t tok = p.gd.div((uint32_t)(live ? row : 0));
+            const uint32_t head = use.at.h * p.gd.d + ((live ? row : 0) - tok * p.gd.d);
+            const uint64_t at = (uint64_t)(use.q.q0 + tok) * p.q_stride + (uint64_t)head * p.head_dim;
+            if constexpr (TERMS == 1) {
+#pragma unroll
+                for (int c = part; c < PIECES; c += 8) {
+                    uint4 w = make_uint4(0, 0, 0, 0);
+                    if (live && c * 8 < (int)p.head_dim)
+                        w = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + at + c * 8);
+                    *reinterpret_cast<uint4 *>(smem + F::RING + r * ROW + ((c ^ (r & 7)) << 4)) = w;
+                }
+            } else {
+                float v[DP / 64][8];
+                float mx = 0.0f;
+#pragma unroll
+                for (int k = 0; k < DP / 64; ++k) {
+                    const int c = part + 8 * k;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[k][e] = 0.0f;
+                    if (live && c * 8 < (int)p.head_dim) raw8_to_float(load_raw8(p.q, at + c * 8, T_F32), T_F32, v[k]);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(v[k][e]));
+                }
+                float back = 1.0f;
+                if constexpr (TYPE == T_F16) {
+                    // scale the row's largest |q| into [1, 2): f16's range then holds both terms
+                    for (int x = 1; x < 8; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                    const int ex = min(max((int)(__float_as_uint(mx) >> 23) - 127, -100), 100);
+                    const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
+                    back = __uint_as_float((uint32_t)(127 + ex) << 23);
+#pragma unroll
+                    for (int k = 0; k < DP / 64; ++k)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[k][e] *= down;
+                }
+                if (part == 0) row_scale[r] = back;
+#pragma unroll
+                for (int term = 0; term < TERMS; ++term)
+#pragma unroll
+                    for (int k = 0; k < DP / 64; ++k) {
+                        const int c = part + 8 * k;
+                        uint4 w;
+                        w.x = split2<TYPE>(v[k][0], v[k][1]);
+                        w.y = split2<TYPE>(v[k][2], v[k][3]);
+                        w.z = split2<TYPE>(v[k][4], v[k][5]);
+                        w.w = split2<TYPE>(v[k][6], v[k][7]);
+                        *reinterpret_cast<uint4 *>(smem + F::RING + term * TR * ROW + r * ROW + ((c ^ (r & 7)) << 4)) = w;
+                    }
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                m[k] = -INFINITY;
+                l[k] = 0.0f;
+                row_limits(p, use.q, min(row0 + (lane >> 2) + 8 * k, rows - 1), row_lo[k], row_hi[k]);
+            }
+            int dummy;
+            row_limits(p, use.q, row0, dummy, all_hi);
+            row_limits(p, use.q, min(row0 + TR, rows) - 1, all_lo, dummy);
+            __syncthreads();
+        }
+        cp_wait<NS - 2>();
+        __syncwarp();
+        fill_next();
+        const int j0 = use.g.lo + use.at.c * KC + warp * WK;
+        if (j0 < use.g.hi) {
+            const uint32_t kb = ring + (i % NS) * F::STAGE, vb = kb + WK * ROW;
+            float s[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+            for (int ks = 0; ks < DP / 16; ++ks) {
+                uint32_t b[4];
+                {  // keys 0-7 | 8-15 by the 16 dims of this step
+                    const int key = (lane & 7) + ((lane >> 4) << 3), c = ks * 2 + ((lane >> 3) & 1);
+                    ldsm4(kb + key * ROW + ((c ^ (key & 7)) << 4), b);
+                }
+#pragma unroll
+                for (int term = 0; term < TERMS; ++term) {
+                    uint32_t a[4];
+                    const int r = lane & 15, c = ks * 2 + (lane >> 4);
+                    ldsm4(qs + term * TR * ROW + r * ROW + ((c ^ (r & 7)) << 4), a);
+                    mma<TYPE>(s[0], a, b[0], b[1]);
+                    mma<TYPE>(s[1], a, b[2], b[3]);
+                }
+            }
+            const bool partial = j0 < all_lo || j0 + WK > all_hi;  // some row does not see some key
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const float sc = TERMS > 1 && TYPE == T_F16 ? p.scale_log2 * row_scale[(lane >> 2) + 8 * k] : p.scale_log2;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float &x = s[t][2 * k + e];
+                        x *= sc;
+                        if (partial) {
+                            const int j = j0 + t * 8 + (lane & 3) * 2 + e;
+                            if (j < row_lo[k] || j >= row_hi[k]) x = -INFINITY;
+                        }
+                    }
+                float mx = fmaxf(fmaxf(s[0][2 * k], s[0][2 * k + 1]), fmaxf(s[1][2 * k], s[1][2 * k + 1]));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                const float mn = fmaxf(m[k], mx);
+                const float ref = mn == -INFINITY ? 0.0f : mn;  // nothing seen yet: every weight below is 0
+                const float al = ex2(m[k] - ref);
+                m[k] = mn;
+                l[k] *= al;
+                if (al != 1.0f) {
+#pragma unroll
+                    for (int d = 0; d < DP / 8; ++d) {
+                        o[d][2 * k] *= al;
+                        o[d][2 * k + 1] *= al;
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float &x = s[t][2 * k + e];
+                        x = ex2(x - ref);
+                        l[k] += x;
+                    }
+            }
+            uint32_t a[TERMS][4];
+#pragma unroll
+            for (int term = 0; term < TERMS; ++term) {
+                a[term][0] = split2<TYPE>(s[0][0], s[0][1]);
+                a[term][1] = split2<TYPE>(s[0][2], s[0][3]);
+                a[term][2] = split2<TYPE>(s[1][0], s[1][1]);
+                a[term][3] = split2<TYPE>(s[1][2], s[1][3]);
+            }
+#pragma unroll
+            for (int dt = 0; dt < DP / 16; ++dt) {
+                uint32_t b[4];
+                const int key = (lane & 7) + (((lane >> 3) & 1) << 3), c = dt * 2 + (lane >> 4);
+                ldsm4t(vb + key * ROW + ((c ^ (key & 7)) << 4), b);
+                if (TERMS > 1 || partial) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) b[x] = finite2<TYPE>(b[x], bad);
+                }
+#pragma unroll
+                for (int term = 0; term < TERMS; ++term) {
+                    mma<TYPE>(o[2 * dt], a[term], b[0], b[1]);
+                    mma<TYPE>(o[2 * dt + 1], a[term], b[2], b[3]);
+                }
+            }
+        }
+        if (use.item_end() || i == n - 1) {
+            // join the warps: common maximum, then the scaled sums warp by warp
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                l[k] += __shfl_xor_sync(0xffffffffu, l[k], 1);
+                l[k] += __shfl_xor_sync(0xffffffffu, l[k], 2);
+                if ((lane & 3) == 0) {
+                    wm[warp][(lane >> 2) + 8 * k] = m[k];
+                    wl[warp][(lane >> 2) + 8 * k] = l[k];
+                }
+            }
+            const bool any_bad = __syncthreads_or(bad);
+            float f[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int r = (lane >> 2) + 8 * k;
+                float mm = wm[0][r];
+                for (int w = 1; w < WARPS; ++w) mm = fmaxf(mm, wm[w][r]);
+                f[k] = ex2(m[k] - (mm == -INFINITY ? 0.0f : mm));
+            }
+            for (int w = 0; w < WARPS; ++w) {
+                if (warp == w) {
+#pragma unroll
+                    for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            float2 *at = reinterpret_cast<float2 *>(osum + ((lane >> 2) + 8 * k) * DP + d * 8 + (lane & 3) * 2);
+                            float2 v = make_float2(o[d][2 * k] * f[k], o[d][2 * k + 1] * f[k]);
+                            if (w) v.x += at->x, v.y += at->y;
+                            *at = v;
+                        }
+                }
+                __syncthreads();
+            }
+            const bool whole = first_c == 0 && use.item_end();
+            float *po = p.part_o + ((size_t)blockIdx.x * 2 + (segment ? 1 : 0)) * TR * DP;
+            float *pm = p.part_ml + ((size_t)blockIdx.x * 2 + (segment ? 1 : 0)) * TR * 2;
+            // eight threads per row, as for the queries
+            const int r = threadIdx.x >> 3, part = threadIdx.x & 7, row = row0 + r;
+            if (row < rows) {
+                float mm = wm[0][r];
+                for (int w = 1; w < WARPS; ++w) mm = fmaxf(mm, wm[w][r]);
+                const float ref = mm == -INFINITY ? 0.0f : mm;
+                float ll = 0.0f;
+                for (int w = 0; w < WARPS; ++w) ll += wl[w][r] * ex2(wm[w][r] - ref);
+                int lo, hi;
+                row_limits(p, use.q, row, lo, hi);
+                const uint32_t tok = p.gd.div((uint32_t)row);
+                const uint32_t head = use.at.h * p.gd.d + (row - tok * p.gd.d);
+                const float inv = whole ? (ll > 0.0f || ll != ll ? 1.0f / ll : 0.0f) : 1.0f;
+                for (int c = part; c * 8 < (int)p.head_dim; c += 8) {
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        v[e] = osum[r * DP + c * 8 + e] * inv;
+                        if (any_bad) {
+                            // the 16-key steps of this segment whose V was cleaned
+                            const int s0 = use.g.lo + first_c * KC, s1 = min(use.g.lo + (use.at.c + 1) * KC, use.g.hi);
+                            for (int j = s0; j < s1; j += WK)
+                                if (TERMS > 1 || j < all_lo || j + WK > all_hi)
+                                    v[e] += nonfinite_v(p, use.at.r, use.at.h, c * 8 + e, j, min(j + WK, s1), lo, hi);
+                        }
+                    }
+                    if (whole)
+                        store8(p.out, (uint64_t)(use.q.q0 + tok) * p.out_stride + (uint64_t)head * p.head_dim + c * 8,
+                               p.io_type, v);
+                    else
+                        store8(po, (uint64_t)r * DP + c * 8, T_F32, v);
+                }
+                if (part == 0) {
+                    if (!whole) {
+                        pm[r * 2] = mm;
+                        pm[r * 2 + 1] = ll;
+                    } else if (p.lse) {
+                        p.lse[(uint64_t)(use.q.q0 + tok) * (p.n_kv * p.gd.d) + head] =
+                            ll > 0.0f || ll != ll ? (mm + log2f(ll)) * LN2 : -INFINITY;
+                    }
+                }
+            }
+            ++segment;
+            fresh = true;
+            __syncthreads();
+        }
+        if (i + 1 < n) use.next(p);
+    }
+    cp_wait<0>();
+}
+
+// Joins the partial results of the items that span CTAs.  Block (j, y) takes the item that boundary
+// j + 1 (the start of CTA j + 1's range) cuts, if it is the item's first cut, and every gridDim.y-th
+// row of its tile.
+template <class S, int TR, int DP>
+__global__ void __launch_bounds__(128) k_attn_join(const AttnParams p, int grid) {
+    __shared__ typename S::Shared sh;
+    grid_dep_trigger_small();
+    grid_dep_wait();
+    long long U;
+    int C;
+    Pos at;
+    Geo g;
+    const int j = (int)blockIdx.x + 1;
+    if (!S::find(p, sh, grid, j, U, C, at, g)) return;
+    const long long u = S::start(U, C, j), a = u - at.c, b = a + g.nch;
+    if (at.c == 0 || S::start(U, C, j - 1) > a) return;  // the cut is an item's start, or not its first
+    const Req q = load_req(p, at.r);
+    const int rows = q.nq * (int)p.gd.d;
+    // CTAs c0 = j - 1 .. c1 hold parts: c0's in its first slot if the item starts its range
+    const int s0 = S::start(U, C, j - 1) == a ? 0 : 1;
+    const auto slot = [&](int c) { return (size_t)c * 2 + (c == j - 1 ? s0 : 0); };
+    const auto holds = [&](int c) { return c < C && S::start(U, C, c) < b; };
+    const int groups = blockDim.x / (DP / 4);  // a thread owns four neighbouring columns of a row
+    const int col = (threadIdx.x % (DP / 4)) * 4;
+    for (int r = (int)blockIdx.y * groups + threadIdx.x / (DP / 4); r < TR; r += gridDim.y * groups) {
+        const int row = at.t * TR + r;
+        if (row >= rows) break;
+        float mm = -INFINITY;
+        for (int c = j - 1; holds(c); ++c) mm = fmaxf(mm, p.part_ml[(slot(c) * TR + r) * 2]);
+        const float ref = mm == -INFINITY ? 0.0f : mm;
+        float ll = 0.0f;
+        float4 o = make_float4(0, 0, 0, 0);
+        for (int c = j - 1; holds(c); ++c) {
+            const float *ml = p.part_ml + (slot(c) * TR + r) * 2;
+            const float w = ex2(ml[0] - ref);
+            const float4 v = *reinterpret_cast<const float4 *>(p.part_o + (slot(c) * TR + r) * DP + col);
+            ll += w * ml[1];
+            o.x += w * v.x;
+            o.y += w * v.y;
+            o.z += w * v.z;
+            o.w += w * v.w;
+        }
+        const bool some = ll > 0.0f || ll != ll;
+        const float inv = some ? 1.0f / ll : 0.0f;
+        const uint32_t tok = p.gd.div((uint32_t)row);
+        const uint32_t head = at.h * p.gd.d + (row - tok * p.gd.d);
+        if (col < (int)p.head_dim) {
+            const uint64_t e = (uint64_t)(q.q0 + tok) * p.out_stride + (uint64_t)head * p.head_dim + col;
+            if (p.io_type == T_F32)
+                *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + e) =
+                    make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+            else
+                *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + e) =
+                    make_uint2(pack2(p.io_type, o.x * inv, o.y * inv), pack2(p.io_type, o.z * inv, o.w * inv));
+        }
+        if (p.lse && col == 0)
+            p.lse[(uint64_t)(q.q0 + tok) * (p.n_kv * p.gd.d) + head] = some ? (mm + log2f(ll)) * LN2 : -INFINITY;
+    }
+}
+
+template <int TYPE, int DP, int TERMS>
+int launch(AttnParams p, cudaStream_t s) {
+    using F = Few<DP, TERMS>;
+    static unsigned long long done = 0;
+    if (attr_pending(done)) {
+        cudaError_t e = cudaFuncSetAttribute(k_attn_few<TYPE, DP, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM);
+        if (e != cudaSuccess) return (int)e;
+        attr_mark(done);
+    }
+    const uint32_t grid = SMS * F::CTAS;
+    p.part_ml = p.part_o + (size_t)grid * 2 * TR * DP;
+    cudaError_t e = launch_pdl(k_attn_few<TYPE, DP, TERMS>, dim3(grid), dim3(WARPS * 32), F::SMEM, s, p);
+    if (e == cudaSuccess) e = launch_pdl(k_attn_join<S, TR, DP>, dim3(grid - 1, 1), dim3(128), 0, s, p, (int)grid);
+    return (int)e;
+}
+template <int TYPE, int DP>
+int launch_terms(const AttnParams &p, cudaStream_t s) {
+    return p.io_type == T_F32 ? launch<TYPE, DP, TYPE == T_BF16 ? 3 : 2>(p, s) : launch<TYPE, DP, 1>(p, s);
+}
+template <int TYPE>
+int launch_dim(const AttnParams &p, cudaStream_t s) {
+    if (p.head_dim <= 64) return launch_terms<TYPE, 64>(p, s);
+    if (p.head_dim <= 128) return launch_terms<TYPE, 128>(p, s);
+    return launch_terms<TYPE, 256>(p, s);
+}
+
+}  // namespace
+}  // namespace attn
+
+size_t attn_few_workspace_bytes(uint32_t head_dim) {
+    const size_t dp = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256, ctas = dp == 64 ? 3 : dp == 128 ? 2 : 1;
+    return SMS * ctas * 2 * attn::TR * (dp + 2) * 4;
+}
+
+int launch_attn_few(const AttnParams &p, cudaStream_t s) {
+    return p.cache_type == T_BF16 ? attn::launch_dim<T_BF16>(p, s) : attn::launch_dim<T_F16>(p, s);
+}
+
+}  // namespace ck

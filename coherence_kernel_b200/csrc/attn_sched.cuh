@@ -1,0 +1,249 @@
+// attn_sched.cuh -- how the attention kernels share their work out over a fixed number of CTAs.
+//
+// An item is one tile of TR rows (rows = tokens x the query heads of one K/V head, token-major) of
+// one request and K/V head; a unit is KC consecutive keys of an item.  Units are numbered request
+// by request, tile by tile, head by head, key chunk by key chunk, and CTA c of C takes units
+// [c U / C, (c + 1) U / C): the split depends on the lengths alone, so ragged batches, one long
+// request and many short ones all fill the GPU evenly and results do not depend on timing.  An
+// item that spans CTAs leaves one partial result per CTA (running maximum, sum, unnormalised
+// output), which a second kernel joins in CTA order.
+//
+// The lengths are device data: every CTA sums the units of all requests itself (a few loads per
+// thread) instead of waiting for a planning kernel.
+#pragma once
+#include "ck_launch.h"
+#include "serve_common.cuh"
+
+namespace ck {
+namespace attn {
+
+struct Req {
+    int q0, nq, kl;  // first row of q, new tokens, visible cache length
+};
+CK_DEV Req load_req(const AttnParams &p, int r) {
+    Req q;
+    const int a = min(max(p.q_start[r], 0), (int)p.ntok), b = min(max(p.q_start[r + 1], a), (int)p.ntok);
+    q.q0 = a;
+    q.nq = b - a;
+    q.kl = (int)min((int64_t)max(p.kv_len[r], 0), (int64_t)p.max_blocks * p.btd.d);
+    return q;
+}
+
+struct Geo {
+    int lo, hi, nch;  // keys [lo, hi) of the tile and its chunks (at least one, so that empty rows are written)
+};
+// Keys a tile of rows [row, row + TR) sees: the last row's upper bound, the first row's lower one.
+template <int TR, int KC>
+CK_DEV Geo tile_geo(const AttnParams &p, const Req &q, int t) {
+    const int rows = q.nq * (int)p.gd.d;
+    const int first = t * TR, last = min(first + TR, rows) - 1;
+    const int base = q.kl - q.nq;  // position of the request's first new token
+    Geo g;
+    g.hi = p.causal ? min(q.kl, base + (int)p.gd.div(last) + 1) : q.kl;
+    g.lo = p.window ? max(0, base + (int)p.gd.div(first) - p.window + 1) & ~15 : 0;
+    if (g.hi <= g.lo) {
+        g.lo = g.hi = 0;
+        g.nch = 1;
+    } else {
+        g.nch = (g.hi - g.lo + KC - 1) / KC;
+    }
+    return g;
+}
+
+struct Pos {
+    int r, t, h, c;
+};
+
+// The kind of request a kernel takes: few rows, or many (CHUNK).
+template <int TR, int KC, bool CHUNK>
+struct Sched {
+    static CK_DEV int tiles(const AttnParams &p, const Req &q) {
+        const int rows = q.nq * (int)p.gd.d;
+        if (CHUNK ? rows < (int)p.row_split : rows >= (int)p.row_split) return 0;
+        return (rows + TR - 1) / TR;
+    }
+    // units of request r (all 32 lanes of a warp call this together, each with its own request)
+    static CK_DEV long long units(const AttnParams &p, int r) {
+        Req q = {0, 0, 0};
+        if (r < (int)p.nreq) q = load_req(p, r);
+        const int nt = r < (int)p.nreq ? tiles(p, q) : 0;
+        long long n = 0;
+        if (nt <= 4)
+            for (int t = 0; t < nt; ++t) n += tile_geo<TR, KC>(p, q, t).nch;
+        // requests of many tiles: the warp's lanes share them out
+        for (uint32_t todo = __ballot_sync(0xffffffffu, nt > 4); todo; todo &= todo - 1) {
+            const int src = __ffs(todo) - 1;
+            const Req w = {0, __shfl_sync(0xffffffffu, q.nq, src), __shfl_sync(0xffffffffu, q.kl, src)};
+            const int wt = __shfl_sync(0xffffffffu, nt, src);
+            int part = 0;
+            for (int t = threadIdx.x & 31; t < wt; t += 32) part += tile_geo<TR, KC>(p, w, t).nch;
+            part = __reduce_add_sync(0xffffffffu, part);
+            if ((int)(threadIdx.x & 31) == src) n = part;
+        }
+        return n * (int)p.n_kv;
+    }
+
+    struct Shared {
+        long long warp_sum[32];
+        long long total, before;
+        Pos pos;
+        Geo geo;
+    };
+    // exclusive prefix of v over the CTA; `all` receives the sum
+    static CK_DEV long long scan(long long v, Shared &sh, long long &all) {
+        const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
+        long long s = v;
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, s, o);
+            if (lane >= o) s += u;
+        }
+        if (lane == 31) sh.warp_sum[w] = s;
+        __syncthreads();
+        long long before = 0;
+        all = 0;
+        for (int i = 0; i < nw; ++i) {
+            if (i < w) before += sh.warp_sum[i];
+            all += sh.warp_sum[i];
+        }
+        __syncthreads();
+        return before + s - v;
+    }
+    static CK_DEV long long start(long long U, int C, int c) { return U * c / C; }
+
+    // Called by the whole CTA.  Finds the total U, the CTAs that take part C = min(grid, U), and the
+    // position of unit start(cta); returns false when cta takes no part.
+    static CK_DEV bool find(const AttnParams &p, Shared &sh, int grid, int cta, long long &U, int &C, Pos &pos, Geo &geo) {
+        const int n = (int)p.nreq, bd = (int)blockDim.x;
+        long long mine = units(p, threadIdx.x), all = 0, sum = mine;
+        for (int b = bd; b < n; b += bd) sum += units(p, b + (int)threadIdx.x);
+        scan(sum, sh, U);
+        C = (int)(U < grid ? U : grid);
+        if (cta >= C) return false;
+        const long long u = start(U, C, cta);
+        long long base = 0;
+        for (int b = 0;; b += bd) {
+            if (b) mine = units(p, b + (int)threadIdx.x);
+            const long long ex = base + scan(mine, sh, all);
+            if (u < base + all) {
+                if (u >= ex && u < ex + mine) {
+                    sh.pos.r = b + (int)threadIdx.x;
+                    sh.before = u - ex;
+                }
+                break;
+            }
+            base += all;
+        }
+        __syncthreads();
+        if (threadIdx.x < 32) {  // the tile of the request: 32 at a time
+            const int lane = threadIdx.x;
+            const int r = sh.pos.r;
+            long long v = sh.before;
+            const Req q = load_req(p, r);
+            const int nt = tiles(p, q);
+            for (int tb = 0; tb < nt; tb += 32) {
+                const int t = tb + lane;
+                Geo g = {0, 0, 0};
+                if (t < nt) g = tile_geo<TR, KC>(p, q, t);
+                const long long m = (long long)g.nch * p.n_kv;
+                long long s = m;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const long long x = __shfl_up_sync(0xffffffffu, s, o);
+                    if (lane >= o) s += x;
+                }
+                const long long tot = __shfl_sync(0xffffffffu, s, 31);
+                if (v < tot) {
+                    if (v >= s - m && v < s) {
+                        const int in = (int)(v - (s - m));
+                        sh.pos.t = t;
+                        sh.pos.h = in / g.nch;
+                        sh.pos.c = in - sh.pos.h * g.nch;
+                        sh.geo = g;
+                    }
+                    break;
+                }
+                v -= tot;
+            }
+        }
+        __syncthreads();
+        pos = sh.pos;
+        geo = sh.geo;
+        return true;
+    }
+
+    // A walk over consecutive units.
+    struct Cursor {
+        Pos at;
+        Req q;
+        Geo g;
+        int nt;
+        CK_DEV void set(const AttnParams &p, const Pos &pos, const Geo &geo) {
+            at = pos;
+            g = geo;
+            q = load_req(p, pos.r);
+            nt = tiles(p, q);
+        }
+        CK_DEV bool item_end() const { return at.c == g.nch - 1; }
+        // the next unit; the caller knows that there is one
+        CK_DEV void next(const AttnParams &p) {
+            if (++at.c < g.nch) return;
+            at.c = 0;
+            if (++at.h < (int)p.n_kv) return;
+            at.h = 0;
+            if (++at.t >= nt) {
+                at.t = 0;
+                do {
+                    if (++at.r >= (int)p.nreq) return;
+                    q = load_req(p, at.r);
+                    nt = tiles(p, q);
+                } while (nt == 0);
+            }
+            g = tile_geo<TR, KC>(p, q, at.t);
+        }
+    };
+};
+
+// The keys that row's token may see: [lo, hi).
+CK_DEV void row_limits(const AttnParams &p, const Req &q, int row, int &lo, int &hi) {
+    const int pos = q.kl - q.nq + (int)p.gd.div((uint32_t)row);
+    hi = p.causal ? min(q.kl, pos + 1) : q.kl;
+    lo = p.window ? max(0, pos - p.window + 1) : 0;
+}
+
+// Element offset of key j of request r in the cache (head 0), or -1 for a page outside the cache.
+CK_DEV int64_t key_offset(const AttnParams &p, int r, int j) {
+    const uint32_t b = p.btd.div((uint32_t)j);
+    const int pg = p.table[(uint64_t)r * p.table_stride + b];
+    if (pg < 0 || pg >= (int)p.n_blocks) return -1;
+    return (int64_t)((uint64_t)pg * p.block_stride + ((uint32_t)j - b * p.btd.d) * p.token_stride);
+}
+
+CK_DEV bool finite16(uint16_t b, int type) {
+    const uint16_t m = type == T_BF16 ? 0x7F80 : 0x7C00;
+    return (b & m) != m;
+}
+CK_DEV float value16(uint16_t b, int type) {
+    return type == T_BF16 ? bf16_bits_to_float(b) : __half2float(__ushort_as_half(b));
+}
+// Where some rows of a tile see a key and others do not, the matrix product takes V's infinities and
+// NaNs as zeros (0 x inf would reach the rows that do not see them); this is what they add to the
+// rows that do: the sum of the non-finite V[j][d] over the visible j of [j0, j1).
+CK_DEV float nonfinite_v(const AttnParams &p, int r, int h, int d, int j0, int j1, int lo, int hi) {
+    float s = 0.0f;
+    for (int j = max(j0, lo); j < min(j1, hi); ++j) {
+        const int64_t at = key_offset(p, r, j);
+        if (at < 0) continue;
+        const uint16_t b = static_cast<const uint16_t *>(p.v)[at + (int64_t)(h * p.head_stride) + d];
+        if (!finite16(b, p.cache_type)) s += value16(b, p.cache_type);
+    }
+    return s;
+}
+
+CK_DEV float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float LN2 = 0.69314718055994531f;
+
+}  // namespace attn
+}  // namespace ck

@@ -11,6 +11,24 @@
 
 namespace ck {
 
+// n / d for 0 <= n < 2^31 by a multiplication: with s = ceil(log2 d) and
+// mul = floor(2^32 (2^s - d) / d) + 1, (mulhi(n, mul) + n) >> s is exact for 32-bit n, and the sum
+// stays below 2^32 for n < 2^31 (the round-up method of Granlund and Montgomery, 1994).
+struct FastDiv {
+    uint32_t mul, shift, d;
+    static FastDiv make(uint32_t d) {
+        FastDiv f;
+        f.d = d;
+        f.shift = 0;
+        while ((1ull << f.shift) < d) ++f.shift;
+        f.mul = (uint32_t)(((1ull << 32) * ((1ull << f.shift) - d)) / d + 1);
+        return f;
+    }
+#ifdef __CUDACC__
+    __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, mul) + n) >> shift; }
+#endif
+};
+
 int launch_q80_dequant(const uint8_t *qb, float *w, uint64_t off, uint64_t n, cudaStream_t s);
 int launch_q4k_dequant(const uint8_t *qb, float *w, uint64_t off, uint64_t n, cudaStream_t s);
 int launch_q4k_dequant_bf16(const uint8_t *qb, void *w, uint64_t off, uint64_t n, cudaStream_t s);
@@ -149,5 +167,53 @@ int launch_gemm_dense(const GemmParams &p, cudaStream_t s);
 // fp32 [rows, k] -> bf16 [rows, 3k]: w = w1 + w2 + w3 with each term the bf16 rounding of the
 // remainder (exact to about 2^-24 relative)
 int launch_split_bf16x3(const float *w, uint16_t *out, uint32_t rows, uint32_t k, cudaStream_t s);
+
+// ---- serving around a paged KV cache.  Element types by GGUF number: 0 f32, 1 f16, 30 bf16, 8 Q8_0.
+// RMS norm with the residual's addition (norm_kernels.cu); strides in elements
+int launch_rmsnorm_add(int x_type, const void *x, uint64_t x_stride, int res_type, const void *res, void *res_out,
+                       uint64_t res_stride, const float *gain, int out_type, void *out, uint64_t out_stride,
+                       uint32_t ntok, uint32_t hidden, float eps, cudaStream_t s);
+// block tables and slot maps from request lengths, and the K/V write (kv_kernels.cu)
+constexpr uint32_t KV_PLAN_MAX_REQUESTS = 16384;  // three running sums per request in shared memory
+struct KvPlanParams {
+    const int32_t *len_in, *new_tokens, *count_in;
+    int32_t *table, *free_blocks;
+    int32_t *len_out, *count_out, *kv_len, *q_start, *positions;
+    int64_t *slots;
+    uint64_t table_stride;
+    uint32_t nreq, ntok, max_blocks, n_blocks;
+    FastDiv btd;  // tokens per page
+};
+int launch_kv_plan(const KvPlanParams &p, cudaStream_t s);
+struct KvAppendParams {
+    const void *k, *v;
+    uint64_t k_stride, v_stride;
+    const int64_t *slots;
+    void *k_cache, *v_cache;
+    uint64_t block_stride, token_stride, head_stride;
+    int64_t n_slots;
+    uint32_t ntok;
+    int cache_type;
+    FastDiv btd, row_div, head_div;  // tokens per page; eight-element pieces per token row and per head
+};
+int launch_kv_append(const KvAppendParams &p, int in_type, cudaStream_t s);
+
+// attention over the paged cache (attn_paged.cu, attn_chunk.cu)
+struct AttnParams {
+    const void *q, *k, *v;
+    void *out;
+    float *lse;
+    const int32_t *table, *kv_len, *q_start;
+    float *part_o, *part_ml;  // partial results of work items that span CTAs
+    uint64_t q_stride, out_stride, table_stride, block_stride, token_stride, head_stride;
+    uint32_t nreq, ntok, n_kv, head_dim, max_blocks, n_blocks;
+    FastDiv btd, gd;     // tokens per page; query heads per K/V head
+    uint32_t row_split;  // requests of at least this many rows (tokens x grouped heads) take the chunk form
+    float scale_log2;    // score scale x log2 e
+    int window, causal;  // window 0: none
+    int io_type, cache_type;
+};
+size_t attn_few_workspace_bytes(uint32_t head_dim);
+int launch_attn_few(const AttnParams &p, cudaStream_t s);
 
 }  // namespace ck

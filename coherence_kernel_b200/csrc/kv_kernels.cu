@@ -1,0 +1,260 @@
+// kv_kernels.cu -- the paged KV cache's bookkeeping: block tables and slot maps from request
+// lengths, built on the device, and the write of new K/V rows through the slot map.
+//
+// A cache is n_blocks pages of block_tokens tokens.  Request r's token at position p lies in page
+// table[r][p / block_tokens] at p % block_tokens; its slot is page * block_tokens + that.  Free pages
+// are a stack: free[0 .. count).
+#include "ck_launch.h"
+#include "serve_common.cuh"
+
+#include <cooperative_groups.h>
+
+namespace ck {
+namespace {
+
+constexpr int PLAN_THREADS = 1024;
+constexpr int SAT = 1 << 30;  // sums saturate here: past every size that is accepted
+
+CK_DEV int sat_add(int a, int b) { return min(a + b, SAT); }
+
+// Inclusive scan of three saturating sums over the CTA; the running carry is returned in place.
+struct Sum3 {
+    int rows, need, back;
+};
+CK_DEV Sum3 add3(Sum3 a, Sum3 b) { return {sat_add(a.rows, b.rows), sat_add(a.need, b.need), sat_add(a.back, b.back)}; }
+CK_DEV Sum3 shfl_up3(Sum3 v, int o) {
+    return {__shfl_up_sync(0xffffffffu, v.rows, o), __shfl_up_sync(0xffffffffu, v.need, o),
+            __shfl_up_sync(0xffffffffu, v.back, o)};
+}
+CK_DEV Sum3 warp_scan3(Sum3 v) {
+    const int lane = threadIdx.x & 31;
+    for (int o = 1; o < 32; o <<= 1) {
+        const Sum3 u = shfl_up3(v, o);
+        if (lane >= o) v = add3(v, u);
+    }
+    return v;
+}
+
+// the number of entries of a non-decreasing array that are <= key
+CK_DEV int upper(const int *a, int n, int key) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (a[mid] <= key) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo;
+}
+
+struct ReqPlan {
+    int len, rows, have, want;  // want: pages after the call if it is served
+    bool fits;                  // its rows and its pages fit the caller's arrays
+};
+CK_DEV ReqPlan req_plan(const KvPlanParams &p, int r, int row_end) {
+    ReqPlan q;
+    const int cap = (int)min((int64_t)p.max_blocks * p.btd.d, (int64_t)SAT);
+    q.len = min(max(p.len_in[r], 0), cap);
+    const int nw = p.new_tokens[r];
+    const int after = (int)min(max((int64_t)q.len + nw, (int64_t)0), (int64_t)SAT);
+    q.rows = max(nw, 0);
+    q.have = (int)p.btd.div((uint32_t)q.len + p.btd.d - 1);
+    q.want = (int)p.btd.div((uint32_t)after + p.btd.d - 1);
+    q.fits = q.rows > 0 && after <= cap && row_end <= (int)p.ntok;
+    return q;
+}
+
+// The request lengths decide everything, so every CTA of the (single) cluster scans all of them --
+// a few loads per thread -- and no CTA waits for another's result.  The sums over the requests
+// (rows, pages needed, pages returned) stay in shared memory, and the rows, the new table entries
+// and the returned pages are each a flat range that the cluster's threads share out evenly, finding
+// an element's request by binary search: one long prompt among a thousand decodes costs no more
+// than its share.  Inputs that alias outputs (len, count) are read before the cluster's barrier and
+// written after it.
+//
+// Taking a page never waits for a push either: the stack with the returned pages on top is read
+// through the request that returned them, whose own table entries this call does not change.
+__global__ void __launch_bounds__(PLAN_THREADS) k_kv_plan(const KvPlanParams p) {
+    extern __shared__ int sm[];
+    int *row_end = sm, *need_end = sm + p.nreq, *back_end = sm + 2 * p.nreq;
+    __shared__ Sum3 warp_sum[PLAN_THREADS / 32];
+    namespace cg = cooperative_groups;
+    grid_dep_trigger_small();
+    grid_dep_wait();
+    const int n = (int)p.nreq;
+    const int count = min(max(p.count_in[0], 0), (int)p.n_blocks);
+    Sum3 carry = {0, 0, 0};
+    for (int base = 0; base < n; base += PLAN_THREADS) {
+        const int r = base + (int)threadIdx.x;
+        Sum3 v = {0, 0, 0};
+        if (r < n) v.rows = min(max(p.new_tokens[r], 0), SAT);
+        // rows first: whether a request's rows fit decides whether its pages count
+        for (int pass = 0; pass < 2; ++pass) {
+            if (pass == 1) {
+                int need = 0, back = 0;
+                if (r < n) {
+                    const ReqPlan q = req_plan(p, r, row_end[r]);
+                    if (q.fits) need = max(q.want - q.have, 0);
+                    if (p.new_tokens[r] < 0) back = q.have - q.want;
+                }
+                v = {0, need, back};
+            }
+            Sum3 w = warp_scan3(v);
+            if ((threadIdx.x & 31) == 31) warp_sum[threadIdx.x >> 5] = w;
+            __syncthreads();
+            Sum3 before = warp_scan3(warp_sum[threadIdx.x & 31]);
+            const int wi = (int)(threadIdx.x >> 5);
+            const Sum3 all = {__shfl_sync(0xffffffffu, before.rows, 31), __shfl_sync(0xffffffffu, before.need, 31),
+                              __shfl_sync(0xffffffffu, before.back, 31)};
+            const int src = max(wi - 1, 0);
+            Sum3 prev = {__shfl_sync(0xffffffffu, before.rows, src), __shfl_sync(0xffffffffu, before.need, src),
+                         __shfl_sync(0xffffffffu, before.back, src)};
+            if (wi == 0) prev = {0, 0, 0};
+            w = add3(add3(w, prev), carry);
+            if (r < n) {
+                if (pass == 0) row_end[r] = w.rows;
+                else need_end[r] = w.need, back_end[r] = w.back;
+            }
+            if (pass == 0) carry.rows = sat_add(carry.rows, all.rows);
+            else carry = add3(carry, Sum3{0, all.need, all.back});
+            __syncthreads();
+        }
+    }
+    const int back = n ? back_end[n - 1] : 0, need = n ? need_end[n - 1] : 0, rows = n ? row_end[n - 1] : 0;
+    const int top = count + back;
+    // requests are served in order while their pages last; the rest of the requests that need pages
+    // get none.  taken: the largest of the running sums that fits
+    int taken = need;
+    if (need > top) {
+        const int k = upper(need_end, n, top);
+        taken = k ? need_end[k - 1] : 0;
+    }
+    const auto served = [&](const ReqPlan &q, int r) {
+        return q.fits && (q.want <= q.have || need_end[r] <= top);
+    };
+    // page number k of this call, counting down from the stack's top
+    const auto page = [&](int k) {
+        const int at = top - 1 - k;
+        if (at < count) return at >= 0 ? p.free_blocks[at] : -1;
+        const int i = at - count, r = upper(back_end, n, i);
+        if (r >= n) return -1;
+        const ReqPlan q = req_plan(p, r, row_end[r]);
+        return p.table[(uint64_t)r * p.table_stride + q.want + (i - (back_end[r] - (q.have - q.want)))];
+    };
+    // every value the writes below depend on that they may overwrite is read before the barrier: the
+    // lengths through req_plan, so each thread's own requests' results are computed here
+    const int gt = (int)(blockIdx.x * PLAN_THREADS + threadIdx.x), gn = (int)(gridDim.x * PLAN_THREADS);
+
+    // slots and positions of the rows
+    const int live = min(rows, (int)p.ntok);
+    for (int t = gt; t < (int)p.ntok; t += gn) {
+        int64_t slot = -1;
+        int pos = -1;
+        if (t < live) {
+            const int r = upper(row_end, n, t);
+            const ReqPlan q = req_plan(p, r, row_end[r]);
+            if (served(q, r)) {
+                pos = q.len + t - (row_end[r] - q.rows);
+                const int b = (int)p.btd.div((uint32_t)pos);
+                const int pg = b < q.have ? p.table[(uint64_t)r * p.table_stride + b]
+                                          : page(need_end[r] - (q.want - q.have) + b - q.have);
+                if (pg >= 0 && pg < (int)p.n_blocks) slot = (int64_t)pg * p.btd.d + (pos - b * (int)p.btd.d);
+            }
+        }
+        p.slots[t] = slot;
+        p.positions[t] = pos;
+    }
+    // new table entries
+    for (int k = gt; k < taken; k += gn) {
+        const int r = upper(need_end, n, k);
+        const ReqPlan q = req_plan(p, r, row_end[r]);
+        p.table[(uint64_t)r * p.table_stride + q.have + (k - (need_end[r] - (q.want - q.have)))] = page(k);
+    }
+    // returned pages that nobody took: pushed above the old top
+    for (int i = gt; i < top - taken - count; i += gn) {
+        const int r = upper(back_end, n, i);
+        const ReqPlan q = req_plan(p, r, row_end[r]);
+        if (count + i < (int)p.n_blocks)
+            p.free_blocks[count + i] =
+                p.table[(uint64_t)r * p.table_stride + q.want + (i - (back_end[r] - (q.have - q.want)))];
+    }
+    for (int r = gt; r <= n; r += gn) p.q_start[r] = r ? min(row_end[r - 1], (int)p.ntok) : 0;
+    // the lengths and the count may be the inputs' own memory: written once every CTA has read them
+    cg::this_cluster().sync();
+    for (int r = gt; r < n; r += gn) {
+        const ReqPlan q = req_plan(p, r, row_end[r]);
+        const int nw = p.new_tokens[r];
+        const bool ok = served(q, r);
+        const int after = (int)max((int64_t)q.len + nw, (int64_t)0);
+        const int len = nw > 0 && !ok ? q.len : after;
+        p.kv_len[r] = nw > 0 && !ok ? 0 : len;
+        p.len_out[r] = len;
+    }
+    if (gt == 0) p.count_out[0] = min(top - taken, (int)p.n_blocks);
+}
+
+// K/V rows into the cache: one thread moves eight elements of one row of K or V per step, so a
+// warp's reads and writes are whole rows of 16-byte pieces.  Nothing is kept between elements: HBM
+// (many rows) or one read-write round trip (few) is the bound.
+template <int IN>
+__global__ void __launch_bounds__(256) k_kv_append(const KvAppendParams p) {
+    grid_dep_trigger_small();
+    grid_dep_wait();
+    const uint32_t vec_row = p.row_div.d;  // eight-element pieces of a token's K (or V)
+    const uint32_t total = 2 * p.ntok * vec_row;
+    for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < total; i += gridDim.x * blockDim.x) {
+        const uint32_t row = p.row_div.div(i), c = i - row * vec_row;
+        const uint32_t t = row >> 1;
+        const bool is_v = row & 1;
+        const int64_t slot = p.slots[t];
+        if (slot < 0 || slot >= p.n_slots) continue;
+        const uint32_t h = p.head_div.div(c), d = (c - h * p.head_div.d) * 8;
+        const Raw8 raw = load_raw8(is_v ? p.v : p.k, (uint64_t)t * (is_v ? p.v_stride : p.k_stride) + c * 8, IN);
+        const uint32_t b = p.btd.div((uint32_t)slot);
+        const uint64_t at = b * p.block_stride + ((uint32_t)slot - b * p.btd.d) * p.token_stride + h * p.head_stride + d;
+        void *cache = is_v ? p.v_cache : p.k_cache;
+        float v[8];
+        raw8_to_float(raw, IN, v);
+        store8(cache, at, p.cache_type, v);
+    }
+}
+
+}  // namespace
+
+int launch_kv_plan(const KvPlanParams &p, cudaStream_t s) {
+    const size_t smem = (size_t)p.nreq * 12;
+    static unsigned long long done = 0;
+    if (attr_pending(done)) {
+        cudaError_t e = cudaFuncSetAttribute(k_kv_plan, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             KV_PLAN_MAX_REQUESTS * 12);
+        if (e != cudaSuccess) return (int)e;
+        attr_mark(done);
+    }
+    // one cluster: 1 CTA while a thread has at most four rows and requests, else 8
+    const uint32_t ctas = p.ntok <= 4 * PLAN_THREADS && p.nreq <= 4 * PLAN_THREADS ? 1 : 8;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = ctas;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(PLAN_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return (int)cudaLaunchKernelEx(&cfg, k_kv_plan, p);
+}
+
+int launch_kv_append(const KvAppendParams &p, int in_type, cudaStream_t s) {
+    const uint32_t want = (2 * p.ntok * p.row_div.d + 255) / 256;
+    const dim3 grid(want < 8 * SMS ? want : 8 * SMS);
+    switch (in_type) {
+        case T_F32: return (int)launch_pdl(k_kv_append<T_F32>, grid, dim3(256), 0, s, p);
+        case T_F16: return (int)launch_pdl(k_kv_append<T_F16>, grid, dim3(256), 0, s, p);
+        default: return (int)launch_pdl(k_kv_append<T_BF16>, grid, dim3(256), 0, s, p);
+    }
+}
+
+}  // namespace ck

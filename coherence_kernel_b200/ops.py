@@ -14,6 +14,9 @@ from . import _lib
 
 Q8_0_BLOCK_BYTES, Q4K_BLOCK_BYTES = 34, 144
 
+# GGUF's numbers of the element types
+TYPE_NUMBERS = {torch.float32: 0, torch.float16: 1, "q8_0": 8, torch.bfloat16: 30}
+
 
 def _stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
@@ -187,3 +190,50 @@ def route_dsv4(logits, bias, nused, wscale):
     _lib.check(_lib.load().ck_route_dsv4_f32(_ptr(logits), _ptr(bias), _ptr(ids), _ptr(wts), ne, nused, wscale, ntok,
                                              _stream()), "ck_route_dsv4_f32")
     return ids, wts
+
+
+def rmsnorm_add(x, residual, gain, eps, out_dtype=None, out=None, residual_out=None):
+    """RMS norm with the residual's addition (ck_rmsnorm_add): s = x + residual (residual None: s = x),
+    out = s / sqrt(mean(s^2) + eps) * gain.  x and residual are [ntok, hidden] (rows may be strided);
+    s is stored to residual_out, by default the residual itself.  out_dtype: f32, f16, bf16 (default x's)
+    or "q8_0", which returns the rows' GGUF blocks as uint8 [ntok, hidden // 32 * 34]."""
+    ntok, hidden = x.shape
+    kinds = (torch.float32, torch.float16, torch.bfloat16)
+    for t, n in ((x, "x"), (residual, "residual"), (residual_out, "residual_out")):
+        if t is None:
+            continue
+        if not t.is_cuda or t.dtype not in kinds:
+            raise ValueError(f"{n} must be a CUDA tensor of f32, f16 or bf16")
+        if tuple(t.shape) != (ntok, hidden) or (hidden > 1 and t.stride(1) != 1) or (ntok > 1 and t.stride(0) < hidden):
+            raise ValueError(f"{n} must be [{ntok}, {hidden}] with contiguous rows")
+        if t.device != x.device:
+            raise ValueError(f"{n} is on {t.device}, x on {x.device}")
+    _dev(gain, "gain", torch.float32, hidden)
+    if residual is None and residual_out is not None:
+        raise ValueError("residual_out without a residual")
+    if residual is not None:
+        residual_out = residual if residual_out is None else residual_out
+        if residual_out.dtype != residual.dtype or (ntok > 1 and residual_out.stride(0) != residual.stride(0)):
+            raise ValueError("residual_out must have the residual's type and row stride")
+    out_dtype = (out.dtype if out is not None else x.dtype) if out_dtype is None else out_dtype
+    if out_dtype not in TYPE_NUMBERS:
+        raise ValueError(f"unsupported out_dtype {out_dtype}")
+    if out_dtype == "q8_0":
+        if out is None:
+            out = torch.empty((ntok, hidden // 32 * Q8_0_BLOCK_BYTES), dtype=torch.uint8, device=x.device)
+        _dev(out, "out", torch.uint8, ntok * (hidden // 32) * Q8_0_BLOCK_BYTES)
+    else:
+        if out is None:
+            out = torch.empty((ntok, hidden), dtype=out_dtype, device=x.device)
+        if tuple(out.shape) != (ntok, hidden) or out.dtype != out_dtype or (hidden > 1 and out.stride(1) != 1) or \
+                (ntok > 1 and out.stride(0) < hidden):
+            raise ValueError(f"out must be {out_dtype} [{ntok}, {hidden}] with contiguous rows")
+    if gain.device != x.device or out.device != x.device:
+        raise ValueError("x, gain and out must be on one device")
+    row = lambda t: 0 if t is None else (t.stride(0) if ntok > 1 else hidden)
+    with torch.cuda.device(x.device):
+        _lib.check(_lib.load().ck_rmsnorm_add(
+            TYPE_NUMBERS[x.dtype], _ptr(x), row(x), 0 if residual is None else TYPE_NUMBERS[residual.dtype],
+            _ptr(residual), _ptr(residual_out), row(residual), _ptr(gain), TYPE_NUMBERS[out_dtype], _ptr(out),
+            0 if out_dtype == "q8_0" else row(out), ntok, hidden, eps, _stream()), "ck_rmsnorm_add")
+    return out

@@ -331,6 +331,89 @@ int ck_ep_group_forward(ck_ep_group *group, const void *x_bf16_dev, uint32_t nto
 int ck_ep_group_status(ck_ep_group *group);
 void ck_ep_group_destroy(ck_ep_group *group);
 
+/* ---- serving around a paged KV cache: norms, block tables, cache writes and attention of a batch of
+ * requests (the reference keeps one request's cache on the host side of its door and dispatches each
+ * token's norm and attention by itself; none of these has a direct counterpart there).
+ * Element types are GGUF's numbers. */
+#define CK_F32 0
+#define CK_F16 1
+#define CK_Q8_0 8
+#define CK_BF16 30
+
+/* RMS norm with the residual's addition.  Per row t < ntok:
+ *   s = x[t] + res[t]  (s = x[t] where res is NULL);  res_out[t] = s in res_type (where not NULL; may be
+ *   res itself);  out[t] = s / sqrt(mean(s^2) + eps) * gain.
+ * x_type, res_type: CK_F32, CK_F16 or CK_BF16.  out_type: the same, or CK_Q8_0 -- GGUF blocks, row after
+ * row: per 32 values d = f16(f32(max|v| / 127)) and codes round(v / d) in -127..127, from v in fp64.  Strides are in elements between rows (out_stride is not read for CK_Q8_0).
+ * A row that holds a NaN, or a block whose scale passes f16's range, has infinite scales: its values read
+ * back as NaN.  hidden % 8 == 0 (32 for CK_Q8_0), hidden <= 16384, strides % 8 == 0 and >= hidden,
+ * pointers 16-byte aligned (a CK_Q8_0 out: 2).  out must not overlap the inputs. */
+int ck_rmsnorm_add(int x_type, const void *x_dev, uint64_t x_stride, int res_type, const void *res_dev,
+                   void *res_out_dev, uint64_t res_stride, const float *gain_dev, int out_type, void *out_dev,
+                   uint64_t out_stride, uint32_t ntok, uint32_t hidden, float eps, void *stream);
+
+/* Block tables and slot maps from request lengths.  A cache is n_blocks pages of block_tokens tokens;
+ * request r's token at position p lies in page table[r * table_stride + p / block_tokens], and its slot is
+ * page * block_tokens + p % block_tokens.  free_blocks[0 .. *count_in) is a stack of free pages.
+ * Request r < nreq holds len_in[r] tokens and gets new_tokens[r] more (>= 0), or drops its last
+ * -new_tokens[r] (all of them where it holds fewer).  Its new rows follow those of request r - 1.
+ *   - Pages of dropped tokens are pushed first: request by request, in block order.
+ *   - Then requests are served in order.  Each page a request needs is popped, in block order, into its
+ *     table row.  Served: its rows end within ntok, its pages within max_blocks, and the pages needed by
+ *     it and the requests before it (of those that fit) are there.  A request that needs no page is not
+ *     held up by the others.  A request that is not served keeps its length and table.
+ * Outputs: len_out[r] the tokens held; kv_len[r] the tokens its new rows attend over (len_out, but 0
+ * where it has rows and is not served); q_start[nreq + 1] the first row of each request (at most ntok);
+ * for every row t < ntok its slot and position, -1 for rows of requests not served and rows past the
+ * last; *count_out the free pages.  len_out may be len_in and count_out count_in: a captured graph then
+ * advances the state at each replay.  Free list entries outside the cache give slots of -1.
+ * nreq <= 16384, ntok < 2^30, max_blocks * block_tokens < 2^30, n_blocks * block_tokens < 2^31;
+ * free_blocks holds n_blocks entries. */
+int ck_kv_plan(const int32_t *len_in_dev, const int32_t *new_tokens_dev, uint32_t nreq, int32_t *table_dev,
+               uint64_t table_stride, uint32_t max_blocks, int32_t *free_blocks_dev, const int32_t *count_in_dev,
+               uint32_t n_blocks, uint32_t block_tokens, uint32_t ntok, int32_t *len_out_dev, int32_t *count_out_dev,
+               int32_t *kv_len_dev, int32_t *q_start_dev, int64_t *slots_dev, int32_t *positions_dev, void *stream);
+
+/* The cache: K and V alike, element (page b, token i of it, head h, d) at b * block_stride +
+ * i * token_stride + h * head_stride + d (strides in elements, each a multiple of 8; base pointers
+ * 16-byte aligned).  cache_type CK_BF16 or CK_F16; head_dim % 8 == 0, head_dim <= 256;
+ * n_blocks * block_tokens < 2^31. */
+typedef struct {
+    uint32_t n_kv_heads, head_dim, block_tokens, n_blocks, cache_type, reserved;
+    uint64_t block_stride, token_stride, head_stride;
+} ck_kv_config;
+
+/* K/V rows k[t], v[t] (n_kv_heads * head_dim elements of in_type -- CK_F32, CK_F16, CK_BF16 -- rows
+ * k_stride, v_stride apart, multiples of 8) into the cache at slots[t], t < ntok, rounded to the cache's
+ * type (f32 beyond f16's range becomes infinite).  Slots outside the cache are skipped.  Slots of one call
+ * have to differ: of two rows with the same slot, either's pieces may stay.
+ * ntok * n_kv_heads * head_dim < 2^32. */
+int ck_kv_append(const ck_kv_config *cfg, int in_type, const void *k_dev, uint64_t k_stride, const void *v_dev,
+                 uint64_t v_stride, const int64_t *slots_dev, uint32_t ntok, void *k_cache_dev, void *v_cache_dev,
+                 void *stream);
+
+/* Attention of each request's new tokens over its cached ones (the new ones among them: append first).
+ * Request r's rows are q[q_start[r] .. q_start[r + 1]), its keys the cache's positions
+ * 0 .. kv_len[r] - 1 through its table row; the last row is at position kv_len[r] - 1, the row before it
+ * one earlier.  A row sees the positions up to its own (causal != 0) or all of them, and of those the last
+ * `window` up to its own (window 0: no bound).
+ *   out[t, h] = sum_j p_j V[j, h'] / sum_j p_j,  p_j = exp(scale q[t, h] . K[j, h']),  h' = h / (n_heads / n_kv_heads)
+ * lse (NULL, or fp32 [ntok, n_heads]) receives log(sum_j p_j).  A row that sees nothing is 0 with lse
+ * -infinity.  Rows q_start[nreq] .. are not touched; lengths beyond the table row or ntok are cut to
+ * them; a table entry outside the cache is read as a page of zeros.  What a row does not see does not
+ * reach it, infinities and NaNs among it (of what it sees: an infinite K element gives NaN in the f32 form).
+ * io_type (q and out): the cache's type, with P rounded to it once before the second product, or CK_F32, which
+ * keeps fp32 accuracy.  q_stride, out_stride: elements between rows, multiples of 8.  n_heads is a multiple
+ * of n_kv_heads; ntok * n_heads < 2^30, max_blocks * block_tokens < 2^30.  ntok bounds the rows:
+ * q_start[nreq] <= ntok.  workspace: ck_paged_attention_workspace_bytes (the same for every batch size); calls that overlap in
+ * time need one each. */
+size_t ck_paged_attention_workspace_bytes(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim);
+int ck_paged_attention(const ck_kv_config *cfg, uint32_t n_heads, int io_type, const void *q_dev, uint64_t q_stride,
+                       const void *k_cache_dev, const void *v_cache_dev, const int32_t *table_dev, uint64_t table_stride,
+                       uint32_t max_blocks, const int32_t *kv_len_dev, const int32_t *q_start_dev, uint32_t nreq,
+                       uint32_t ntok, float scale, int causal, uint32_t window, void *out_dev, uint64_t out_stride,
+                       float *lse_dev, void *workspace_dev, size_t workspace_bytes, void *stream);
+
 /* Failure-path self-test (no counterpart in the reference).  Runs the library's bounded device wait
  * on an mbarrier that nothing ever arrives on, with a time limit of limit_ns (1 ns .. 2 s): the wait
  * gives up, writes code 77 to *err_dev (which the caller zeroes first) and the time it waited to
