@@ -115,6 +115,7 @@ SIGNATURES = {
     "ck_kv_plan": (_i32, [_p, _p, _u32, _p, _u64, _u32, _p, _p, _u32, _u32, _u32, _p, _p, _p, _p, _p, _p, _p]),
     "ck_kv_append": (_i32, [ctypes.POINTER(KvConfig), _i32, _p, _u64, _p, _u64, _p, _u32, _p, _p, _p]),
     "ck_paged_attention_workspace_bytes": (_sz, [_u32, _u32, _u32]),
+    "ck_paged_attention_status": (_i32, [_p, _p]),
     "ck_paged_attention": (_i32, [ctypes.POINTER(KvConfig), _u32, _i32, _p, _u64, _p, _p, _p, _u64, _u32, _p, _p,
                                   _u32, _u32, _f, _i32, _u32, _p, _u64, _p, _p, _sz, _p]),
     # the handle door

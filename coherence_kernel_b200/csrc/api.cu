@@ -600,7 +600,20 @@ int ck_kv_append(const ck_kv_config *c, int in_type, const void *k, uint64_t k_s
 size_t ck_paged_attention_workspace_bytes(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim) {
     if (n_heads == 0 || n_kv_heads == 0 || n_heads % n_kv_heads || head_dim == 0 || head_dim % 8 || head_dim > 256)
         return 0;
-    return al(ck::attn_few_workspace_bytes(head_dim));
+    return 256 + al(ck::attn_few_workspace_bytes(head_dim)) + al(ck::attn_chunk_workspace_bytes(head_dim));
+}
+
+int ck_paged_attention_status(const void *ws, void *s) {
+    if (!ws) return fail(CK_EARG, "ck_paged_attention_status");
+    int e = 0;
+    cudaError_t r = cudaMemcpyAsync(&e, ws, 4, cudaMemcpyDeviceToHost, S(s));
+    if (r == cudaSuccess) r = cudaStreamSynchronize(S(s));
+    if (r != cudaSuccess) return fail((int)r, "ck_paged_attention_status");
+    if (e) {
+        snprintf(g_err, sizeof(g_err), "ck_paged_attention: device wait timed out (role code %d)", e);
+        return CK_ETIMEOUT;
+    }
+    return 0;
 }
 
 int ck_paged_attention(const ck_kv_config *c, uint32_t n_heads, int io_type, const void *q, uint64_t q_stride,
@@ -615,6 +628,7 @@ int ck_paged_attention(const ck_kv_config *c, uint32_t n_heads, int io_type, con
         (uint64_t)max_blocks * c->block_tokens >= 1u << 30 || nreq >= 1u << 30)
         return fail(CK_ESHAPE, "ck_paged_attention");
     if (io_type != CK_F32 && io_type != (int)c->cache_type) return fail(CK_EARG, "ck_paged_attention type");
+    if (!(scale > 0.0f && scale < 3.0e38f)) return fail(CK_EARG, "ck_paged_attention scale");
     if (nreq == 0 || ntok == 0) return 0;
     if (!q || !out || !k_cache || !v_cache || !table || !kv_len || !q_start || !ws || off16(q) || off16(out) ||
         off16(k_cache) || off16(v_cache) || off16(ws))
@@ -632,7 +646,7 @@ int ck_paged_attention(const ck_kv_config *c, uint32_t n_heads, int io_type, con
     p.table = table;
     p.kv_len = kv_len;
     p.q_start = q_start;
-    p.part_o = (float *)ws;
+    p.err = (int *)ws;
     p.q_stride = q_stride;
     p.out_stride = out_stride;
     p.table_stride = table_stride;
@@ -647,13 +661,23 @@ int ck_paged_attention(const ck_kv_config *c, uint32_t n_heads, int io_type, con
     p.n_blocks = c->n_blocks;
     p.btd = ck::FastDiv::make(c->block_tokens);
     p.gd = ck::FastDiv::make(n_heads / c->n_kv_heads);
-    p.row_split = 0x7fffffffu;
     p.scale_log2 = scale * 1.44269504088896341f;
     // a window as long as the table row bounds nothing
     p.window = window >= (uint64_t)max_blocks * c->block_tokens ? 0 : (int)window;
     p.causal = causal;
     p.io_type = io_type;
     p.cache_type = (int)c->cache_type;
+    // requests of many rows take the chunk form, where any can have that many; the others the few-row
+    // form in a launch of its own
+    const bool chunk = ck::attn_chunk_ok_types(io_type, (int)c->cache_type, c->head_dim) &&
+                       (uint64_t)ntok * p.gd.d >= ck::ATTN_CHUNK_ROWS;
+    p.row_split = chunk ? ck::ATTN_CHUNK_ROWS : ck::ATTN_NO_CHUNK;
+    if (chunk) {
+        p.part_o = (float *)((uint8_t *)ws + 256 + al(ck::attn_few_workspace_bytes(c->head_dim)));
+        rc = ck::launch_attn_chunk(p, S(s));
+        if (rc) return fail(rc, "ck_paged_attention");
+    }
+    p.part_o = (float *)((uint8_t *)ws + 256);
     return fail(ck::launch_attn_few(p, S(s)), "ck_paged_attention");
 }
 

@@ -245,5 +245,65 @@ CK_DEV float ex2(float x) {
 }
 constexpr float LN2 = 0.69314718055994531f;
 
+// Joins the partial results of the items that span CTAs.  Block (j, y) takes the item that boundary
+// j + 1 (the start of CTA j + 1's range) cuts, if it is the item's first cut, and every gridDim.y-th
+// row of its tile.
+template <class S, int TR, int DP>
+__global__ void __launch_bounds__(128) k_attn_join(const AttnParams p, int grid) {
+    __shared__ typename S::Shared sh;
+    grid_dep_trigger_small();
+    grid_dep_wait();
+    long long U;
+    int C;
+    Pos at;
+    Geo g;
+    const int j = (int)blockIdx.x + 1;
+    if (!S::find(p, sh, grid, j, U, C, at, g)) return;
+    const long long u = S::start(U, C, j), a = u - at.c, b = a + g.nch;
+    if (at.c == 0 || S::start(U, C, j - 1) > a) return;  // the cut is an item's start, or not its first
+    const Req q = load_req(p, at.r);
+    const int rows = q.nq * (int)p.gd.d;
+    // CTAs c0 = j - 1 .. c1 hold parts: c0's in its first slot if the item starts its range
+    const int s0 = S::start(U, C, j - 1) == a ? 0 : 1;
+    const auto slot = [&](int c) { return (size_t)c * 2 + (c == j - 1 ? s0 : 0); };
+    const auto holds = [&](int c) { return c < C && S::start(U, C, c) < b; };
+    const int groups = blockDim.x / (DP / 4);  // a thread owns four neighbouring columns of a row
+    const int col = (threadIdx.x % (DP / 4)) * 4;
+    for (int r = (int)blockIdx.y * groups + threadIdx.x / (DP / 4); r < TR; r += gridDim.y * groups) {
+        const int row = at.t * TR + r;
+        if (row >= rows) break;
+        float mm = -INFINITY;
+        for (int c = j - 1; holds(c); ++c) mm = fmaxf(mm, p.part_ml[(slot(c) * TR + r) * 2]);
+        const float ref = mm == -INFINITY ? 0.0f : mm;
+        float ll = 0.0f;
+        float4 o = make_float4(0, 0, 0, 0);
+        for (int c = j - 1; holds(c); ++c) {
+            const float *ml = p.part_ml + (slot(c) * TR + r) * 2;
+            const float w = ex2(ml[0] - ref);
+            const float4 v = *reinterpret_cast<const float4 *>(p.part_o + (slot(c) * TR + r) * DP + col);
+            ll += w * ml[1];
+            o.x += w * v.x;
+            o.y += w * v.y;
+            o.z += w * v.z;
+            o.w += w * v.w;
+        }
+        const bool some = ll > 0.0f || ll != ll;
+        const float inv = some ? 1.0f / ll : 0.0f;
+        const uint32_t tok = p.gd.div((uint32_t)row);
+        const uint32_t head = at.h * p.gd.d + (row - tok * p.gd.d);
+        if (col < (int)p.head_dim) {
+            const uint64_t e = (uint64_t)(q.q0 + tok) * p.out_stride + (uint64_t)head * p.head_dim + col;
+            if (p.io_type == T_F32)
+                *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + e) =
+                    make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+            else
+                *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + e) =
+                    make_uint2(pack2(p.io_type, o.x * inv, o.y * inv), pack2(p.io_type, o.z * inv, o.w * inv));
+        }
+        if (p.lse && col == 0)
+            p.lse[(uint64_t)(q.q0 + tok) * (p.n_kv * p.gd.d) + head] = some ? (mm + log2f(ll)) * LN2 : -INFINITY;
+    }
+}
+
 }  // namespace attn
 }  // namespace ck

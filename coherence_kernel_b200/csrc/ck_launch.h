@@ -205,6 +205,7 @@ struct AttnParams {
     float *lse;
     const int32_t *table, *kv_len, *q_start;
     float *part_o, *part_ml;  // partial results of work items that span CTAs
+    int *err;                 // device error word (bounded waits)
     uint64_t q_stride, out_stride, table_stride, block_stride, token_stride, head_stride;
     uint32_t nreq, ntok, n_kv, head_dim, max_blocks, n_blocks;
     FastDiv btd, gd;     // tokens per page; query heads per K/V head
@@ -215,5 +216,11 @@ struct AttnParams {
 };
 size_t attn_few_workspace_bytes(uint32_t head_dim);
 int launch_attn_few(const AttnParams &p, cudaStream_t s);
+constexpr uint32_t ATTN_CHUNK_ROWS = 64, ATTN_NO_CHUNK = 0x7fffffffu;
+inline bool attn_chunk_ok_types(int io_type, int cache_type, uint32_t head_dim) {
+    return io_type == cache_type && head_dim <= 128;
+}
+size_t attn_chunk_workspace_bytes(uint32_t head_dim);
+int launch_attn_chunk(const AttnParams &p, cudaStream_t s);
 
 }  // namespace ck

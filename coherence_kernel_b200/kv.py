@@ -170,6 +170,10 @@ class PagedAttention:
                 _ptr(lse), _ptr(self.ws), self.ws_bytes, _stream()), "ck_paged_attention")
         return (out, lse) if return_lse else out
 
+    def status(self):
+        """Synchronize and raise if a device-side wait of the last call gave up."""
+        _lib.check(_lib.load().ck_paged_attention_status(_ptr(self.ws), _stream()), "ck_paged_attention_status")
+
 
 class PagedKV:
     """A paged KV cache with its state on the device: pages, request lengths, tables, free pages."""

@@ -404,7 +404,7 @@ int ck_kv_append(const ck_kv_config *cfg, int in_type, const void *k_dev, uint64
  * reach it, infinities and NaNs among it (of what it sees: an infinite K element gives NaN in the f32 form).
  * io_type (q and out): the cache's type, with P rounded to it once before the second product, or CK_F32, which
  * keeps fp32 accuracy.  q_stride, out_stride: elements between rows, multiples of 8.  n_heads is a multiple
- * of n_kv_heads; ntok * n_heads < 2^30, max_blocks * block_tokens < 2^30.  ntok bounds the rows:
+ * of n_kv_heads, scale finite and > 0; ntok * n_heads < 2^30, max_blocks * block_tokens < 2^30.  ntok bounds the rows:
  * q_start[nreq] <= ntok.  workspace: ck_paged_attention_workspace_bytes (the same for every batch size); calls that overlap in
  * time need one each. */
 size_t ck_paged_attention_workspace_bytes(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim);
@@ -413,6 +413,9 @@ int ck_paged_attention(const ck_kv_config *cfg, uint32_t n_heads, int io_type, c
                        uint32_t max_blocks, const int32_t *kv_len_dev, const int32_t *q_start_dev, uint32_t nreq,
                        uint32_t ntok, float scale, int causal, uint32_t window, void *out_dev, uint64_t out_stride,
                        float *lse_dev, void *workspace_dev, size_t workspace_bytes, void *stream);
+/* After a ck_paged_attention call with this workspace: synchronizes `stream` and returns CK_ETIMEOUT when a
+ * device-side wait gave up (out is then not valid), else 0. */
+int ck_paged_attention_status(const void *workspace_dev, void *stream);
 
 /* Failure-path self-test (no counterpart in the reference).  Runs the library's bounded device wait
  * on an mbarrier that nothing ever arrives on, with a time limit of limit_ns (1 ns .. 2 s): the wait

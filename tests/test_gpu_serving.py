@@ -247,6 +247,7 @@ def run_attn(q, k, v, table, kl, starts, scale, pad=0, **kw):
     out = torch.full_like(qq, 77.0)
     lse = torch.full((q.shape[0] + pad, nh), 77.0, device="cuda")
     at(qq, k.cuda(), v.cuda(), i(table), i(kl), i(starts), scale, out=out, lse=lse, **kw)
+    at.status()
     assert (out[q.shape[0]:] == 77.0).all() and (lse[q.shape[0]:] == 77.0).all()
     return out[:q.shape[0]].cpu(), lse[:q.shape[0]].cpu()
 
@@ -283,6 +284,41 @@ def test_attention_chunks(cache, io, heads, kv_heads, dim, bt):
     check_attn(attn_case(bt, lens, heads, kv_heads, dim, bt, cache, io, width_slack=2), pad=5)
 
 
+CHUNK_LENS = [[(63, 63), (64, 64), (65, 65)], [(200, 127), (300, 128), (129, 129), (2, 1)],
+              [(255, 255), (700, 256), (257, 257)], [(1500, 300)], [(0, 0), (900, 40), (5, 5), (400, 150)]]
+
+
+@pytest.mark.parametrize("lens", CHUNK_LENS)
+@pytest.mark.parametrize("cache", [BF16, F16])
+@pytest.mark.parametrize("heads,kv_heads,dim,bt", [(2, 2, 128, 16), (1, 1, 64, 24), (3, 1, 96, 128), (2, 1, 8, 1)])
+def test_attention_chunk_form(lens, cache, heads, kv_heads, dim, bt):
+    check_attn(attn_case(dim + len(lens), lens, heads, kv_heads, dim, bt, cache, cache), pad=2)
+
+
+@pytest.mark.parametrize("window,causal", [(1, True), (33, True), (200, True), (200, False), (0, False)])
+def test_attention_chunk_form_masks(window, causal):
+    check_attn(attn_case(window, [(500, 400), (300, 70)], 2, 2, 64, 16, BF16, BF16), causal=causal, window=window)
+    case = list(attn_case(3, [(200, 150), (130, 130)], 2, 1, 128, 16, BF16, BF16))
+    case[4] = [20, 0]  # most rows before the cache's start; a request that is not served
+    check_attn(tuple(case), causal=causal, window=window)
+
+
+def test_attention_chunk_form_many_heads_over_one():
+    check_attn(attn_case(3, [(300, 1), (77, 1), (1, 1), (513, 2)], 128, 1, 128, 16, BF16, BF16))
+
+
+def test_attention_chunk_form_growing_scores():
+    """Scores that keep growing along the keys: every unit moves the running maximum past the rescaling step."""
+    q, k, v, table, kl, starts = attn_case(3, [(1400, 150)], 2, 2, 64, 16, F16, F16)
+    order = torch.arange(1400)
+    for b, pg in enumerate(table[0]):
+        n = min(16, 1400 - b * 16)
+        k[pg, :n] = (k[pg, :n] * 0.1 + (order[b * 16:b * 16 + n].view(-1, 1, 1) / 1400)).to(F16)
+    q = (q.abs() * 2).to(F16)
+    check_attn((q, k, v, table, kl, starts), scale=1.0)
+    check_attn((-q, k, v, table, kl, starts), scale=1.0)
+
+
 @pytest.mark.parametrize("window", [1, 5, 16, 64, 100, 10 ** 9])
 @pytest.mark.parametrize("causal", [True, False])
 def test_attention_windows_and_no_causal_bound(window, causal):
@@ -314,6 +350,36 @@ def test_attention_many_requests():
     rng = random.Random(4)
     lens = [(rng.randrange(1, 60), 1) if r % 7 else (rng.randrange(20, 90), rng.randrange(0, 20)) for r in range(700)]
     check_attn(attn_case(5, lens, 2, 1, 64, 16, BF16, BF16))
+
+
+def test_attention_chunk_form_takes_nothing_from_what_is_not_seen():
+    lens = [(300, 260), (150, 100)]
+    q, k, v, table, kl, starts = attn_case(6, lens, 2, 2, 64, 16, BF16, BF16)
+    used = {p for r, (l, _) in enumerate(lens) for p in table[r][:-(-l // 16)]}
+    for p in range(k.shape[0]):
+        if p not in used:
+            k[p], v[p] = math.nan, math.inf
+    for r, (l, _) in enumerate(lens):
+        if l % 16:
+            k[table[r][l // 16], l % 16:], v[table[r][l // 16], l % 16:] = math.nan, math.nan
+    base = (q, k, v, table, kl, starts)
+    check_attn(base)
+    clean, _ = run_attn(*base, 0.125)
+    for pos, bad in ((30, math.inf), (100, -math.inf), (170, math.nan), (299, math.inf)):
+        v2, k2 = v.clone(), k.clone()
+        v2[table[0][pos // 16], pos % 16, 1, 5] = bad
+        k2[table[1][5], 9, 0, 0] = math.nan  # position 89 of request 1
+        out, _ = run_attn(q, k2, v2, table, kl, starts, 0.125)
+        first = max(pos - 40, 0)
+        other = torch.ones(64, dtype=torch.bool)
+        other[5] = False
+        assert torch.equal(out[:first], clean[:first])
+        hit = out[first:260, 1, 5]
+        assert (torch.isnan(hit) if math.isnan(bad) else hit == bad).all()
+        assert torch.equal(out[first:260][:, :, other], clean[first:260][:, :, other])
+        assert torch.equal(out[:260, 0], clean[:260, 0])
+        assert torch.equal(out[260:299], clean[260:299]) and torch.isnan(out[299:, 0]).all()
+        assert torch.equal(out[299:, 1], clean[299:, 1])
 
 
 @pytest.mark.parametrize("io", [BF16, F32])

@@ -103,7 +103,8 @@ def test_attention_bad_configs(cuda_lib, kw, rc):
     (dict(q=P + 8), EARG), (dict(out=P + 2), EARG), (dict(kc=None), EARG), (dict(vc=P + 1), EARG), (dict(table=None), EARG),
     (dict(kl=None), EARG), (dict(st=None), EARG), (dict(ws=None), EARG), (dict(wsb=16), EARG), (dict(qs=248), EARG),
     (dict(os=260), EARG), (dict(ts=4), EARG), (dict(mb=0), ESHAPE), (dict(mb=1 << 27, ts=1 << 27), ESHAPE),
-    (dict(ntok=1 << 28), ESHAPE)])
+    (dict(ntok=1 << 28), ESHAPE), (dict(scale=0.0), EARG), (dict(scale=-1.0), EARG),
+    (dict(scale=float("nan")), EARG), (dict(scale=float("inf")), EARG)])
 def test_attention_refusals(cuda_lib, kw, rc):
     assert attend(cuda_lib, **kw) == rc
     assert b"ck_paged_attention" in cuda_lib.ck_last_error()
