@@ -600,7 +600,8 @@ int ck_kv_append(const ck_kv_config *c, int in_type, const void *k, uint64_t k_s
 size_t ck_paged_attention_workspace_bytes(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim) {
     if (n_heads == 0 || n_kv_heads == 0 || n_heads % n_kv_heads || head_dim == 0 || head_dim % 8 || head_dim > 256)
         return 0;
-    return 256 + al(ck::attn_few_workspace_bytes(head_dim)) + al(ck::attn_chunk_workspace_bytes(head_dim));
+    return 256 + 2 * al(sizeof(ck::AttnCuts)) + al(ck::attn_few_workspace_bytes(head_dim)) +
+           al(ck::attn_chunk_workspace_bytes(head_dim));
 }
 
 int ck_paged_attention_status(const void *ws, void *s) {
@@ -667,17 +668,24 @@ int ck_paged_attention(const ck_kv_config *c, uint32_t n_heads, int io_type, con
     p.causal = causal;
     p.io_type = io_type;
     p.cache_type = (int)c->cache_type;
-    // requests of many rows take the chunk form, where any can have that many; the others the few-row
-    // form in a launch of its own
-    const bool chunk = ck::attn_chunk_ok_types(io_type, (int)c->cache_type, c->head_dim) &&
+    // Requests of many rows take the chunk form, the others the few-row form in a launch of its own.  A batch
+    // with no more rows than requests is a decode step, and its requests have one row each (or padding): only
+    // the few-row form is launched, unless a single token's heads already fill a chunk tile's threshold.
+    const bool decode = ntok <= nreq && p.gd.d < ck::ATTN_CHUNK_ROWS;
+    const bool chunk = !decode && ck::attn_chunk_ok_types(io_type, (int)c->cache_type, c->head_dim) &&
                        (uint64_t)ntok * p.gd.d >= ck::ATTN_CHUNK_ROWS;
     p.row_split = chunk ? ck::ATTN_CHUNK_ROWS : ck::ATTN_NO_CHUNK;
+    uint8_t *at = (uint8_t *)ws + 256;  // after the error word: each form's cuts, then its parts
+    const auto take = [&](size_t bytes) { uint8_t *b = at; at += al(bytes); return b; };
+    p.cuts = (ck::AttnCuts *)take(sizeof(ck::AttnCuts));
+    p.part_o = (float *)take(ck::attn_few_workspace_bytes(c->head_dim));
     if (chunk) {
-        p.part_o = (float *)((uint8_t *)ws + 256 + al(ck::attn_few_workspace_bytes(c->head_dim)));
-        rc = ck::launch_attn_chunk(p, S(s));
+        ck::AttnParams g = p;
+        g.cuts = (ck::AttnCuts *)take(sizeof(ck::AttnCuts));
+        g.part_o = (float *)take(ck::attn_chunk_workspace_bytes(c->head_dim));
+        rc = ck::launch_attn_chunk(g, S(s));
         if (rc) return fail(rc, "ck_paged_attention");
     }
-    p.part_o = (float *)((uint8_t *)ws + 256);
     return fail(ck::launch_attn_few(p, S(s)), "ck_paged_attention");
 }
 

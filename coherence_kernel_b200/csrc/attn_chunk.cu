@@ -106,8 +106,27 @@ CK_DEV void item_limits(const AttnParams &p, const Req &q, int t, int &all_lo, i
     row_limits(p, q, min(t * TR + TR, rows) - 1, all_lo, dummy);
 }
 
+CK_DEV float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// What V's infinities and NaNs, taken as zeros in the units that some row of the item sees in part, add to one
+// row's columns d0 .. d0 + 15.
+__device__ __noinline__ void add_nonfinite(const AttnParams &p, const Pos &at, const Req &q, const Geo &g, int c0, int c1,
+                                           int d0, int lo, int hi, float (&v)[16]) {
+    int all_lo, all_hi;
+    item_limits(p, q, at.t, all_lo, all_hi);
+    for (int c = c0; c < c1; ++c) {
+        const int j = g.lo + c * KC;
+        if (j >= all_lo && j + KC <= all_hi) continue;
+        for (int x = 0; x < 16; ++x)
+            if (d0 + x < (int)p.head_dim) v[x] += nonfinite_v(p, at.r, at.h, d0 + x, j, min(j + KC, g.hi), lo, hi);
+    }
+}
+
 template <int TYPE, int DP>
-__global__ void __launch_bounds__(NTHREADS, 1) k_attn_chunk(const AttnParams p) {
+__global__ void __launch_bounds__(NTHREADS, 1) k_attn_chunk(const __grid_constant__ AttnParams p) {
     using F = Chunk<DP>;
     constexpr int PIECES = DP / 8;           // 16-byte pieces of a row
     constexpr int ROWS_PER = 32 / PIECES;    // rows one warp instruction copies
@@ -127,7 +146,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) k_attn_chunk(const AttnParams p) 
     int C;
     Pos pos;
     Geo geo;
-    if (!S::find(p, sh, (int)gridDim.x, (int)blockIdx.x, U, C, pos, geo)) return;
+    const bool part = S::find(p, sh, (int)gridDim.x, (int)blockIdx.x, U, C, pos, geo);
+    S::leave_cut(p, U, C, pos, geo);
+    if (!part) return;
     const int n = (int)(S::start(U, C, blockIdx.x + 1) - S::start(U, C, blockIdx.x));
     if (threadIdx.x == 0) {
         for (int i = 0; i < NS; ++i) {
@@ -158,14 +179,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) k_attn_chunk(const AttnParams p) 
         // -------------------------------------------------------------------------------- loader
         reg_dec<80>();
         const int w = warp - 8;
-        typename S::Cursor at;
-        at.set(p, pos, geo);
-        // lane l holds key 32 w + l of a unit: its element offset, -1 to fill with zeros
-        const auto lookup = [&]() -> int64_t {
-            const int j = at.g.lo + at.at.c * KC + w * 32 + lane;
-            if (j >= at.g.hi) return -1;
-            const int64_t o = key_offset(p, at.at.r, j);
-            return o < 0 ? -1 : o + (int64_t)(at.at.h * p.head_stride);
+        typename S::Items it;
+        it.set(p, pos, geo, n);
+        // lane l holds key 32 w + l of unit c: its element offset, -1 to fill with zeros
+        const auto lookup = [&](int c) -> int64_t {
+            const int j = it.g.lo + c * KC + w * 32 + lane;
+            if (j >= it.g.hi) return -1;
+            const int64_t o = key_offset(p, it.at.r, j);
+            return o < 0 ? -1 : o + (int64_t)(it.at.h * p.head_stride);
         };
         // 32 rows of a tile by this warp
         const auto copy_rows = [&](uint32_t tile, int row0, const void *base, int64_t off) {
@@ -233,60 +254,52 @@ __global__ void __launch_bounds__(NTHREADS, 1) k_attn_chunk(const AttnParams p) 
             const bool ok = mbar_wait_bounded(b, parity, p.err, 30);
             return __all_sync(0xffffffffu, ok);
         };
-        uint32_t e = 0, item = 0;
-        int64_t off = lookup();
-        bool fresh = true, ok = true;
-        int all_lo = 0, all_hi = 0;
-        for (int i = 0; i < n && ok; ++i) {
-            const int64_t cur = off;
-            const Pos here = at.at;
-            const Req q = at.q;
-            const int j0 = at.g.lo + at.at.c * KC;
-            const bool ends = at.item_end();
-            if (fresh) item_limits(p, q, here.t, all_lo, all_hi);
-            const bool partial = j0 < all_lo || j0 + KC > all_hi;
-            if (i + 1 < n) {
-                at.next(p);
-                off = lookup();
-            }
-            // K
-            uint32_t st = e % NS, tile = sbase + F::RING_OFF + st * F::TILE;
-            ok = room(&bar->empty[st], ((e / NS) & 1) ^ 1);
-            if (!ok) break;
-            copy_rows(tile, w * 32, p.k, cur);
-            push(&bar->full[st], 0, 0);
-            ++e;
-            if (fresh) {  // the item's query rows
-                ok = room(&bar->q_empty, (item & 1) ^ 1);
+        uint32_t e = 0, item = 0;  // ring entries and items so far
+        bool ok = true;
+        do {
+            int all_lo, all_hi;
+            item_limits(p, it.q, it.at.t, all_lo, all_hi);
+            int64_t next = lookup(it.c0);
+            for (int c = it.c0; c < it.c1 && ok; ++c) {
+                const int64_t off = next;
+                if (c + 1 < it.c1) next = lookup(c + 1);
+                const int j0 = it.g.lo + c * KC;
+                const bool partial = j0 < all_lo || j0 + KC > all_hi;
+                // K
+                uint32_t st = e % NS, tile = sbase + F::RING_OFF + st * F::TILE;
+                ok = room(&bar->empty[st], ((e / NS) & 1) ^ 1);
                 if (!ok) break;
-                const int rows = q.nq * (int)p.gd.d;
-                for (int b = 0; b < 2; ++b) {
-                    const int lr = w * 64 + b * 32 + lane, row = here.t * TR + lr;
-                    int64_t o = -1;
-                    if (row < rows) {
-                        const uint32_t tok = p.gd.div((uint32_t)row);
-                        o = (int64_t)((uint64_t)(q.q0 + tok) * p.q_stride +
-                                      (uint64_t)(here.h * p.gd.d + row - tok * p.gd.d) * p.head_dim);
+                copy_rows(tile, w * 32, p.k, off);
+                push(&bar->full[st], 0, 0);
+                ++e;
+                if (c == it.c0) {  // the item's query rows
+                    ok = room(&bar->q_empty, (item & 1) ^ 1);
+                    if (!ok) break;
+                    const int rows = it.q.nq * (int)p.gd.d;
+                    for (int b = 0; b < 2; ++b) {
+                        const int row = it.at.t * TR + w * 64 + b * 32 + lane;
+                        int64_t o = -1;
+                        if (row < rows) {
+                            const uint32_t tok = p.gd.div((uint32_t)row);
+                            o = (int64_t)((uint64_t)(it.q.q0 + tok) * p.q_stride +
+                                          (uint64_t)(it.at.h * p.gd.d + row - tok * p.gd.d) * p.head_dim);
+                        }
+                        // rows 0-127 and 128-255 are a tile each
+                        copy_rows(sbase + F::Q_OFF + (w >> 1) * F::TILE, (w & 1) * 64 + b * 32, p.q, o);
                     }
-                    // rows 0-127 and 128-255 are a tile each
-                    copy_rows(sbase + F::Q_OFF + (w >> 1) * F::TILE, (w & 1) * 64 + b * 32, p.q, o);
+                    push(&bar->q_full, 0, 0);
                 }
-                push(&bar->q_full, 0, 0);
-                fresh = false;
+                // V
+                st = e % NS;
+                tile = sbase + F::RING_OFF + st * F::TILE;
+                ok = room(&bar->empty[st], ((e / NS) & 1) ^ 1);
+                if (!ok) break;
+                copy_rows(tile, w * 32, p.v, off);
+                push(&bar->full[st], partial ? tile : 0, item + 1);
+                ++e;
             }
-            // V
-            st = e % NS;
-            tile = sbase + F::RING_OFF + st * F::TILE;
-            ok = room(&bar->empty[st], ((e / NS) & 1) ^ 1);
-            if (!ok) break;
-            copy_rows(tile, w * 32, p.v, cur);
-            push(&bar->full[st], partial ? tile : 0, item + 1);
-            ++e;
-            if (ends) {
-                fresh = true;
-                ++item;
-            }
-        }
+            ++item;
+        } while (ok && it.next(p));
         drain();
     } else if (wg == 3) {
         // ---------------------------------------------------------------------------- the products
@@ -294,29 +307,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) k_attn_chunk(const AttnParams p) 
         if (warp == 12) {
             constexpr uint32_t id_s = idesc16(TYPE, 128, KC, 0), id_o = idesc16(TYPE, 128, DP, 1);
             constexpr uint32_t HALF = F::TILE / F::HALVES;
-            typename S::Cursor at;
-            at.set(p, pos, geo);
-            const auto scores = [&](int t, uint32_t ktile) {
-                if (elect_one()) {
-#pragma unroll
-                    for (int k = 0; k < DP / 16; ++k) {
-                        const uint32_t o = (k >> 2) * HALF + (k & 3) * 32;
-                        umma_bf16(tmem + s_col(t), sdesc_k_sw128(sbase + F::Q_OFF + t * F::TILE + o),
-                                  sdesc_k_sw128(ktile + o), id_s, k != 0);
-                    }
-                    umma_commit(&bar->s_full[t]);
-                }
-                __syncwarp();
-            };
-            const auto values = [&](int t, uint32_t vtile, bool first) {
-                if (elect_one()) {
-#pragma unroll
-                    for (int k = 0; k < KC / 16; ++k)
-                        umma_bf16_ts(tmem + o_col(t), tmem + s_col(t) + k * 8, sdesc_n_sw128(vtile + k * 2048, HALF), id_o,
-                                     !(first && k == 0));
-                }
-                __syncwarp();
-            };
+            const uint64_t q_desc = sdesc_k_sw128(sbase + F::Q_OFF), k_desc = sdesc_k_sw128(sbase + F::RING_OFF),
+                           v_desc = sdesc_n_sw128(sbase + F::RING_OFF, HALF);
+            constexpr uint32_t STAGE16 = F::TILE >> 4;  // descriptors count 16 bytes
+            typename S::Items it;
+            it.set(p, pos, geo, n);
             const auto commit = [&](uint64_t *b) {
                 if (elect_one()) umma_commit(b);
                 __syncwarp();
@@ -327,50 +322,59 @@ __global__ void __launch_bounds__(NTHREADS, 1) k_attn_chunk(const AttnParams p) 
                 tc_fence_after();
                 return all;
             };
-            const auto tile = [&](uint32_t e) { return sbase + F::RING_OFF + (e % NS) * F::TILE; };
-            // entries of the ring: unit i's K is 2 i, its V 2 i + 1
-            uint32_t item = 0, handed[2] = {0, 0};  // P tiles taken from each softmax warpgroup
-            int nh = halves(p, at.q, at.at.t);
-            const auto unit_scores = [&](int t, int i) {  // S_t of unit i (the cursor's)
-                const uint32_t ek = 2 * i;
-                scores(t, tile(ek));
-                if (t == nh - 1) {
-                    commit(&bar->empty[ek % NS]);
-                    if (at.item_end() || i == n - 1) commit(&bar->q_empty);
-                }
-            };
-            bool ok = wait(&bar->q_full, 0, 31) && wait(&bar->full[0], 0, 32);
-            for (int t = 0; t < nh && ok; ++t) unit_scores(t, 0);
-            bool first = true;
-            for (int i = 0; i < n && ok; ++i) {
-                const bool last = at.item_end() || i == n - 1;  // the item's last unit in this CTA
-                const uint32_t ev = 2 * i + 1, ek = 2 * i + 2;
-                ok = wait(&bar->full[ev % NS], (ev / NS) & 1, 33);
-                for (int t = 0; t < nh && ok; ++t) {
-                    ok = wait(&bar->p_full[t], handed[t] & 1, 34);
-                    if (!ok) break;
-                    ++handed[t];
-                    values(t, tile(ev), first);
-                    if (last) commit(&bar->o_full[t]);
-                    if (t == nh - 1) commit(&bar->empty[ev % NS]);
-                    if (!last) {
-                        if (t == 0) {
-                            ok = wait(&bar->full[ek % NS], (ek / NS) & 1, 35);
-                            if (!ok) break;
-                            at.next(p);
-                        }
-                        unit_scores(t, i + 1);
+            // S_t = Q_t K^T from ring stage st; free: barriers of what this was the last use of
+            const auto scores = [&](int t, uint32_t st, bool k_done, bool q_done) {
+                const uint64_t qd = q_desc + t * STAGE16, kd = k_desc + st * STAGE16;
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k) {
+                        const uint32_t o = (k >> 2) * (HALF >> 4) + (k & 3) * 2;
+                        umma_bf16(tmem + s_col(t), qd + o, kd + o, id_s, k != 0);
                     }
+                    umma_commit(&bar->s_full[t]);
+                    if (k_done) umma_commit(&bar->empty[st]);
+                    if (q_done) umma_commit(&bar->q_empty);
                 }
-                first = last;
-                if (ok && last && i + 1 < n) {
-                    ++item;
-                    at.next(p);
-                    nh = halves(p, at.q, at.at.t);
-                    ok = wait(&bar->q_full, item & 1, 36) && wait(&bar->full[ek % NS], (ek / NS) & 1, 37);
-                    for (int t = 0; t < nh && ok; ++t) unit_scores(t, i + 1);
+                __syncwarp();
+            };
+            // O_t (+)= P_t V from ring stage st
+            const auto values = [&](int t, uint32_t st, bool first, bool v_done, bool o_done) {
+                const uint64_t vd = v_desc + st * STAGE16;
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < KC / 16; ++k)
+                        umma_bf16_ts(tmem + o_col(t), tmem + s_col(t) + k * 8, vd + k * 128, id_o, !(first && k == 0));
+                    if (v_done) umma_commit(&bar->empty[st]);
+                    if (o_done) umma_commit(&bar->o_full[t]);
                 }
-            }
+                __syncwarp();
+            };
+            uint32_t e = 0, item = 0, handed[2] = {0, 0};  // ring entries, items, P tiles taken from each half
+            bool ok = true;
+            do {
+                const int nh = halves(p, it.q, it.at.t), units = it.c1 - it.c0;
+                ok = wait(&bar->q_full, item & 1, 31) && wait(&bar->full[e % NS], (e / NS) & 1, 32);
+                if (!ok) break;
+                for (int t = 0; t < nh; ++t) scores(t, e % NS, t == nh - 1, t == nh - 1 && units == 1);
+                ++e;
+                for (int c = 0; c < units && ok; ++c) {
+                    const bool last = c == units - 1;
+                    const uint32_t sv = e % NS, sk = (e + 1) % NS;
+                    ok = wait(&bar->full[sv], (e / NS) & 1, 33);
+                    for (int t = 0; t < nh && ok; ++t) {
+                        ok = wait(&bar->p_full[t], handed[t] & 1, 34);
+                        if (!ok) break;
+                        ++handed[t];
+                        values(t, sv, c == 0, t == nh - 1, last);
+                        if (!last) {
+                            if (t == 0) ok = wait(&bar->full[sk], ((e + 1) / NS) & 1, 35);
+                            if (ok) scores(t, sk, t == nh - 1, t == nh - 1 && c == units - 2);
+                        }
+                    }
+                    e += last ? 1 : 2;
+                }
+                ++item;
+            } while (ok && it.next(p));
             // every product has completed before tensor memory is freed, also after a wait gave up
             commit(&bar->done);
             mbar_wait_bounded(&bar->done, 0, nullptr, 0);
@@ -381,166 +385,190 @@ __global__ void __launch_bounds__(NTHREADS, 1) k_attn_chunk(const AttnParams p) 
         const int t = wg, r = threadIdx.x & 127;  // tile of the item, row of the tile
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 lanes: lane number << 16
         const uint32_t s_at = tmem + s_col(t) + lanes, o_at = tmem + o_col(t) + lanes;
-        typename S::Cursor at;
-        at.set(p, pos, geo);
-        uint32_t item = 0, taken = 0, joined = 0;  // items met; score tiles and outputs taken
-        int segment = 0, first_c = 0;
-        bool fresh = true, ok = true;
-        float m = -INFINITY, l = 0.0f;
-        int lo = 0, hi = 0, all_lo = 0, all_hi = 0;
-        for (int i = 0; i < n; ++i) {
-            const int rows = at.q.nq * (int)p.gd.d, row0 = at.at.t * TR + t * 128;
-            if (row0 >= rows) {  // no rows in this half: its products are not issued
-                if (at.item_end()) {
-                    ++segment;
-                    ++item;
-                }
-                if (i + 1 < n) at.next(p);
-                continue;
-            }
-            if (fresh) {
-                first_c = at.at.c;
-                m = -INFINITY;
-                l = 0.0f;
+        typename S::Items it;
+        it.set(p, pos, geo, n);
+        uint32_t taken = 0, joined = 0;  // score tiles and outputs taken
+        uint32_t item = 0;
+        int segment = 0;
+        bool ok = true;
+        do {
+            const int rows = it.q.nq * (int)p.gd.d, row0 = it.at.t * TR + t * 128;
+            const size_t slot = (size_t)blockIdx.x * 2 + (segment ? 1 : 0);
+            ++segment;
+            ++item;
+            if (row0 >= rows) continue;  // no rows in this half: its products are not issued
+            int lo, hi, all_lo, all_hi;
+            float m = -INFINITY, l = 0.0f;
+            {
                 int dummy;
-                row_limits(p, at.q, min(row0 + r, rows - 1), lo, hi);
-                row_limits(p, at.q, row0, dummy, all_hi);
-                row_limits(p, at.q, min(row0 + 128, rows) - 1, all_lo, dummy);
+                row_limits(p, it.q, min(row0 + r, rows - 1), lo, hi);
+                row_limits(p, it.q, row0, dummy, all_hi);
+                row_limits(p, it.q, min(row0 + 128, rows) - 1, all_lo, dummy);
             }
-            ok = mbar_wait_bounded(&bar->s_full[t], taken & 1, p.err, 38);
-            if (!__all_sync(0xffffffffu, ok)) break;
-            ++taken;
-            tc_fence_after();
-            uint32_t s[4][32];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld32(s_at + c * 32, s[c]);
-            tmem_ld_wait();
-            const int j0 = at.g.lo + at.at.c * KC;
-            if (j0 < all_lo || j0 + KC > all_hi) {
-                const int a = lo - j0, b = hi - j0;
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-#pragma unroll
-                    for (int x = 0; x < 32; ++x)
-                        if (c * 32 + x < a || c * 32 + x >= b) s[c][x] = 0xFF800000u;  // -infinity
-            }
-            float mx[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                mx[c] = __uint_as_float(s[c][0]);
-#pragma unroll
-                for (int x = 1; x < 32; ++x) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][x]));
-            }
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
-            if (fresh) {
-                m = top;
-            } else {
-                const bool grow = top > m + GROW || (m == -INFINITY && top > m);
-                if (__any_sync(0xffffffffu, grow)) {
-                    // S_t(i) completed, so PV_t(i - 1) has too: O is at rest until P_t(i) is handed over
-                    const float mn = grow ? top : m;
-                    const float al = grow ? ex2(m - mn) : 1.0f;
-                    m = mn;
-                    l *= al;
-#pragma unroll 1
-                    for (int c = 0; c < DP / 32; ++c) {
-                        uint32_t o[32];
-                        tmem_ld32(o_at + c * 32, o);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * al);
-                        tmem_st32(o_at + c * 32, o);
-                    }
-                }
-            }
-            const float ref = m == -INFINITY ? 0.0f : m;
-            const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), rf2 = make_float2(-ref, -ref);
-            float2 sum[2] = {make_float2(0, 0), make_float2(0, 0)};
-#pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-                uint32_t pk[32];
-#pragma unroll
-                for (int x = 0; x < 32; ++x) {
-                    const int c = hh * 2 + x / 16, y = (x % 16) * 2;
-                    float2 v = make_float2(__uint_as_float(s[c][y]), __uint_as_float(s[c][y + 1]));
-                    v = __ffma2_rn(v, sc2, rf2);
-                    v.x = ex2(v.x);
-                    v.y = ex2(v.y);
-                    sum[x & 1] = __fadd2_rn(sum[x & 1], v);
-                    pk[x] = pack2(TYPE, v.x, v.y);
-                }
-                tmem_st32(s_at + hh * 32, pk);
-            }
-            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-            tmem_st_wait();
-            tc_fence_before();
-            mbar_arrive(&bar->p_full[t]);
-            fresh = false;
-            if (at.item_end() || i == n - 1) {
-                ok = mbar_wait_bounded(&bar->o_full[t], joined & 1, p.err, 39);
-                if (!__all_sync(0xffffffffu, ok)) break;
-                ++joined;
+            int j0 = it.g.lo + it.c0 * KC;
+            for (int c = it.c0; c < it.c1; ++c, j0 += KC) {
+                ok = mbar_wait_bounded(&bar->s_full[t], taken & 1, p.err, 38);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                ++taken;
                 tc_fence_after();
-                const bool whole = first_c == 0 && at.item_end();
-                const size_t slot = (size_t)blockIdx.x * 2 + (segment ? 1 : 0);
-                const int row = row0 + r;
-                const bool live = row < rows;
-                const bool cleaned = poison[item & 7] == item + 1;
-                const bool some = l > 0.0f || l != l;
-                const float inv = whole ? (some ? 1.0f / l : 0.0f) : 1.0f;
-                const uint32_t tok = p.gd.div((uint32_t)(live ? row : 0));
-                const uint32_t head = at.at.h * p.gd.d + ((live ? row : 0) - tok * p.gd.d);
-                const uint64_t oe = (uint64_t)(at.q.q0 + tok) * p.out_stride + (uint64_t)head * p.head_dim;
-                float *po = p.part_o + (slot * TR + t * 128 + r) * DP;
+                uint32_t s[4][32];
+#pragma unroll
+                for (int b = 0; b < 4; ++b) tmem_ld32(s_at + b * 32, s[b]);
+                tmem_ld_wait();
+                if (j0 < all_lo || j0 + KC > all_hi) {
+                    const int a = lo - j0, z = hi - j0;
+#pragma unroll
+                    for (int b = 0; b < 4; ++b)
+#pragma unroll
+                        for (int x = 0; x < 32; ++x)
+                            if (b * 32 + x < a || b * 32 + x >= z) s[b][x] = 0xFF800000u;  // -infinity
+                }
+                float mx[4];
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    mx[b] = __uint_as_float(s[b][0]);
+#pragma unroll
+                    for (int x = 1; x + 1 < 32; x += 2) mx[b] = max3(mx[b], __uint_as_float(s[b][x]), __uint_as_float(s[b][x + 1]));
+                }
+                const float top = fmaxf(max3(max3(mx[0], __uint_as_float(s[0][31]), __uint_as_float(s[1][31])), mx[1],
+                                             __uint_as_float(s[2][31])),
+                                        max3(mx[2], mx[3], __uint_as_float(s[3][31]))) *
+                                  p.scale_log2;
+                if (c == it.c0) {
+                    m = top;
+                } else {
+                    const bool grow = top > m + GROW || (m == -INFINITY && top > m);
+                    if (__any_sync(0xffffffffu, grow)) {
+                        // S_t of this unit completed, so PV_t of the last one has too: O is at rest until P_t is
+                        // handed over
+                        const float mn = grow ? top : m;
+                        const float al = grow ? ex2(m - mn) : 1.0f;
+                        m = mn;
+                        l *= al;
 #pragma unroll 1
-                for (int c = 0; c < DP / 32; ++c) {
-                    uint32_t o[32];
-                    tmem_ld32(o_at + c * 32, o);
-                    tmem_ld_wait();
+                        for (int b = 0; b < DP / 16; ++b) {
+                            uint32_t o[16];
+                            tmem_ld16(o_at + b * 16, o);
+                            tmem_ld_wait();
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const int d = c * 32 + g * 8;
-                        if (!live || d >= (int)p.head_dim) continue;
-                        float v[8];
-#pragma unroll
-                        for (int x = 0; x < 8; ++x) v[x] = __uint_as_float(o[g * 8 + x]) * inv;
-                        if (cleaned) {
-                            int il, ih;
-                            item_limits(p, at.q, at.at.t, il, ih);
-                            const int s0 = at.g.lo + first_c * KC, s1 = min(at.g.lo + (at.at.c + 1) * KC, at.g.hi);
-                            for (int j = s0; j < s1; j += KC)
-                                if (j < il || j + KC > ih)
-                                    for (int x = 0; x < 8; ++x)
-                                        v[x] += nonfinite_v(p, at.at.r, at.at.h, d + x, j, min(j + KC, s1), lo, hi);
+                            for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * al);
+                            tmem_st16(o_at + b * 16, o);
                         }
-                        if (whole) store8(p.out, oe + d, TYPE, v);
-                        else store8(po, d, T_F32, v);
-                    }
-                    __syncwarp();
-                }
-                if (live) {
-                    if (!whole) {
-                        float *pm = p.part_ml + (slot * TR + t * 128 + r) * 2;
-                        pm[0] = m;
-                        pm[1] = l;
-                    } else if (p.lse) {
-                        p.lse[(uint64_t)(at.q.q0 + tok) * (p.n_kv * p.gd.d) + head] =
-                            some ? (m + log2f(l)) * LN2 : -INFINITY;
                     }
                 }
+                const float ref = m == -INFINITY ? 0.0f : m;
+                const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), rf2 = make_float2(-ref, -ref);
+                float2 sum[2] = {make_float2(0, 0), make_float2(0, 0)};
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) {
+                        float2 v = make_float2(__uint_as_float(s[b][2 * x]), __uint_as_float(s[b][2 * x + 1]));
+                        v = __ffma2_rn(v, sc2, rf2);
+                        v.x = ex2(v.x);
+                        v.y = ex2(v.y);
+                        sum[x & 1] = __fadd2_rn(sum[x & 1], v);
+                        pk[x] = pack2(TYPE, v.x, v.y);
+                    }
+                    tmem_st16(s_at + b * 16, pk);
+                }
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                tmem_st_wait();
                 tc_fence_before();
-                ++segment;
-                ++item;
-                fresh = true;
+                mbar_arrive(&bar->p_full[t]);
             }
-            if (i + 1 < n) at.next(p);
-        }
+            if (!ok) break;
+            ok = mbar_wait_bounded(&bar->o_full[t], joined & 1, p.err, 39);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            ++joined;
+            tc_fence_after();
+            const bool whole = it.whole();
+            const int row = row0 + r;
+            const bool live = row < rows;
+            const bool some = l > 0.0f || l != l;
+            const float inv = whole ? (some ? 1.0f / l : 0.0f) : 1.0f;
+            const uint32_t tok = p.gd.div((uint32_t)(live ? row : 0));
+            const uint32_t head = it.at.h * p.gd.d + ((live ? row : 0) - tok * p.gd.d);
+            const uint64_t oe = (uint64_t)(it.q.q0 + tok) * p.out_stride + (uint64_t)head * p.head_dim;
+            // a part's column d of all rows is contiguous: a warp's store is one line
+            float *po = p.part_o + slot * (TR * DP) + t * 128 + r;
+            const bool cleaned = poison[(item - 1) & 7] == item;
+#pragma unroll 1
+            for (int b = 0; b < DP / 16; ++b) {
+                uint32_t o[16];
+                tmem_ld16(o_at + b * 16, o);
+                tmem_ld_wait();
+                float v[16];
+#pragma unroll
+                for (int x = 0; x < 16; ++x) v[x] = __uint_as_float(o[x]) * inv;
+                if (cleaned && live) add_nonfinite(p, it.at, it.q, it.g, it.c0, it.c1, b * 16, lo, hi, v);
+                if (!whole) {
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) po[(b * 16 + x) * TR] = v[x];
+                } else if (live) {
+#pragma unroll
+                    for (int g = 0; g < 2; ++g)
+                        if (b * 16 + g * 8 < (int)p.head_dim) {
+                            const float w[8] = {v[g * 8], v[g * 8 + 1], v[g * 8 + 2], v[g * 8 + 3],
+                                                v[g * 8 + 4], v[g * 8 + 5], v[g * 8 + 6], v[g * 8 + 7]};
+                            store8(p.out, oe + b * 16 + g * 8, TYPE, w);
+                        }
+                }
+                __syncwarp();
+            }
+            if (!whole) {
+                float *pm = p.part_ml + slot * (TR * 2) + t * 128 + r;
+                pm[0] = m;
+                pm[TR] = l;
+            } else if (live && p.lse) {
+                p.lse[(uint64_t)(it.q.q0 + tok) * (p.n_kv * p.gd.d) + head] = some ? (m + log2f(l)) * LN2 : -INFINITY;
+            }
+            tc_fence_before();
+        } while (it.next(p));
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     if (warp == 12) tmem_dealloc(tmem, 512);
+}
+
+// Joins the parts of an item that spans CTAs: block (j, y) takes eight columns of all rows of the item whose first
+// cut is boundary j + 1, a thread a row, so that reads of a part's columns are whole lines.
+template <int DP>
+__global__ void __launch_bounds__(TR) k_attn_join_chunk(const __grid_constant__ AttnParams p) {
+    grid_dep_trigger_small();
+    grid_dep_wait();
+    Joint jt;
+    const int d = (int)blockIdx.y * 8;
+    if (d >= (int)p.head_dim || !find_joint(p, (int)blockIdx.x + 1, jt)) return;
+    const Req q = load_req(p, jt.at.r);
+    const int r = threadIdx.x, row = jt.at.t * TR + r;
+    if (row >= q.nq * (int)p.gd.d) return;
+    float mm = -INFINITY;
+    for (int i = 0; i < jt.n; ++i) mm = fmaxf(mm, p.part_ml[jt.slot(i) * (TR * 2) + r]);
+    const float ref = mm == -INFINITY ? 0.0f : mm;
+    float ll = 0.0f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 2
+    for (int i = 0; i < jt.n; ++i) {
+        const size_t at = jt.slot(i);
+        const float w = ex2(p.part_ml[at * (TR * 2) + r] - ref);
+        ll += w * p.part_ml[at * (TR * 2) + TR + r];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) o[x] += w * p.part_o[at * (TR * DP) + (d + x) * TR + r];
+    }
+    const bool some = ll > 0.0f || ll != ll;
+    const float inv = some ? 1.0f / ll : 0.0f;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) o[x] *= inv;
+    const uint32_t tok = p.gd.div((uint32_t)row);
+    const uint32_t head = jt.at.h * p.gd.d + (row - tok * p.gd.d);
+    store8(p.out, (uint64_t)(q.q0 + tok) * p.out_stride + (uint64_t)head * p.head_dim + d, p.io_type, o);
+    if (p.lse && d == 0)
+        p.lse[(uint64_t)(q.q0 + tok) * (p.n_kv * p.gd.d) + head] = some ? (mm + log2f(ll)) * LN2 : -INFINITY;
 }
 
 template <int TYPE, int DP>
@@ -555,7 +583,7 @@ int launch(AttnParams p, cudaStream_t s) {
     const uint32_t grid = SMS;
     p.part_ml = p.part_o + (size_t)grid * 2 * TR * DP;
     cudaError_t e = launch_pdl(k_attn_chunk<TYPE, DP>, dim3(grid), dim3(NTHREADS), F::SMEM, s, p);
-    if (e == cudaSuccess) e = launch_pdl(k_attn_join<S, TR, DP>, dim3(grid - 1, 8), dim3(128), 0, s, p, (int)grid);
+    if (e == cudaSuccess) e = launch_pdl(k_attn_join_chunk<DP>, dim3(grid - 1, DP / 8), dim3(TR), 0, s, p);
     return (int)e;
 }
 

@@ -98,7 +98,7 @@ CK_DEV uint32_t finite2(uint32_t w, bool &bad) {
 }
 
 template <int TYPE, int DP, int TERMS>
-__global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(const AttnParams p) {
+__global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(const __grid_constant__ AttnParams p) {
     using F = Few<DP, TERMS>;
     constexpr int ROW = F::ROW, NS = F::STAGES, PIECES = DP / 8, COPIES = WK * PIECES / 32;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -114,16 +114,19 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
     int C;
     Pos pos;
     Geo geo;
-    if (!S::find(p, sh, (int)gridDim.x, (int)blockIdx.x, U, C, pos, geo)) return;
+    const bool part = S::find(p, sh, (int)gridDim.x, (int)blockIdx.x, U, C, pos, geo);
+    S::leave_cut(p, U, C, pos, geo);
+    if (!part) return;
     const int n = (int)(S::start(U, C, blockIdx.x + 1) - S::start(U, C, blockIdx.x));
-    typename S::Cursor use, fill;
-    use.set(p, pos, geo);
+    typename S::Items use, fill;
+    use.set(p, pos, geo, n);
     fill = use;
+    int fill_c = fill.c0;
 
     // lane l < 16 looks up key l of the warp's next 16: its element offset, or -1 to fill with zeros
     // (past the tile's last key, so that what the page holds there never meets a product)
     const auto lookup = [&]() -> int64_t {
-        const int j = fill.g.lo + fill.at.c * KC + warp * WK + (lane & 15);
+        const int j = fill.g.lo + fill_c * KC + warp * WK + (lane & 15);
         if (j >= fill.g.hi) return -1;
         const int64_t at = key_offset(p, fill.at.r, j);
         return at < 0 ? -1 : at + (int64_t)(fill.at.h * p.head_stride);
@@ -147,7 +150,10 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
         if (filled < n) {
             copy_in(filled % NS, off);
             if (++filled < n) {
-                fill.next(p);
+                if (++fill_c == fill.c1) {
+                    fill.next(p);
+                    fill_c = 0;
+                }
                 off = lookup();
             }
         }
@@ -155,21 +161,17 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
     };
     for (int i = 0; i < NS - 1; ++i) fill_next();
 
-    float o[DP / 8][4];
-    float m[2], l[2];
-    int row_lo[2], row_hi[2];
-    int all_lo = 0, all_hi = 0;  // keys that every row of the tile sees
-    bool bad = false;
-    bool fresh = true;
-    int first_c = 0, segment = 0;
-    for (int i = 0; i < n; ++i) {
+    int i = 0;  // units done
+    for (int segment = 0;; ++segment) {
         const int rows = use.q.nq * (int)p.gd.d, row0 = use.at.t * TR;
-        if (fresh) {
-            fresh = false;
-            first_c = use.at.c;
-            bad = false;
+        float o[DP / 8][4];
+        float m[2], l[2];
+        int row_lo[2], row_hi[2];
+        int all_lo, all_hi;  // keys [all_lo, all_hi) every row of the tile sees
+        bool bad = false;
 #pragma unroll
-            for (int d = 0; d < DP / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.0f;
+        for (int d = 0; d < DP / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.0f;
+        {
             // the query tile: eight threads per row
             const int r = threadIdx.x >> 3, part = threadIdx.x & 7, row = row0 + r;
             const bool live = row < rows;
@@ -233,11 +235,12 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
             row_limits(p, use.q, min(row0 + TR, rows) - 1, all_lo, dummy);
             __syncthreads();
         }
-        cp_wait<NS - 2>();
-        __syncwarp();
-        fill_next();
-        const int j0 = use.g.lo + use.at.c * KC + warp * WK;
-        if (j0 < use.g.hi) {
+        for (int c = use.c0; c < use.c1; ++c, ++i) {
+            cp_wait<NS - 2>();
+            __syncwarp();
+            fill_next();
+            const int j0 = use.g.lo + c * KC + warp * WK;
+            if (j0 >= use.g.hi) continue;
             const uint32_t kb = ring + (i % NS) * F::STAGE, vb = kb + WK * ROW;
             float s[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
@@ -319,7 +322,7 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
                 }
             }
         }
-        if (use.item_end() || i == n - 1) {
+        {
             // join the warps: common maximum, then the scaled sums warp by warp
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -353,7 +356,7 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
                 }
                 __syncthreads();
             }
-            const bool whole = first_c == 0 && use.item_end();
+            const bool whole = use.whole();
             float *po = p.part_o + ((size_t)blockIdx.x * 2 + (segment ? 1 : 0)) * TR * DP;
             float *pm = p.part_ml + ((size_t)blockIdx.x * 2 + (segment ? 1 : 0)) * TR * 2;
             // eight threads per row, as for the queries
@@ -376,7 +379,7 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
                         v[e] = osum[r * DP + c * 8 + e] * inv;
                         if (any_bad) {
                             // the 16-key steps of this segment whose V was cleaned
-                            const int s0 = use.g.lo + first_c * KC, s1 = min(use.g.lo + (use.at.c + 1) * KC, use.g.hi);
+                            const int s0 = use.g.lo + use.c0 * KC, s1 = min(use.g.lo + use.c1 * KC, use.g.hi);
                             for (int j = s0; j < s1; j += WK)
                                 if (TERMS > 1 || j < all_lo || j + WK > all_hi)
                                     v[e] += nonfinite_v(p, use.at.r, use.at.h, c * 8 + e, j, min(j + WK, s1), lo, hi);
@@ -398,13 +401,78 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
                     }
                 }
             }
-            ++segment;
-            fresh = true;
-            __syncthreads();
         }
-        if (i + 1 < n) use.next(p);
+        if (!use.next(p)) break;
+        __syncthreads();
     }
     cp_wait<0>();
+}
+
+// Joins the parts of an item that spans CTAs: block (j, r) takes row r of the item whose first cut is
+// boundary j + 1.  A thread owns four neighbouring columns of every GROUPS-th part; the maximum comes first, so the parts'
+// loads are independent, and the groups' sums are added in a fixed order.
+template <int DP>
+__global__ void __launch_bounds__(128) k_attn_join_few(const __grid_constant__ AttnParams p) {
+    constexpr int COLS = DP / 4, GROUPS = 128 / COLS;
+    __shared__ float red[4];
+    __shared__ float4 sum[GROUPS][COLS];
+    __shared__ float lsum[GROUPS];
+    grid_dep_trigger_small();
+    grid_dep_wait();
+    Joint jt;
+    if (!find_joint(p, (int)blockIdx.x + 1, jt)) return;
+    const Req q = load_req(p, jt.at.r);
+    const int r = (int)blockIdx.y, row = jt.at.t * TR + r;
+    if (row >= q.nq * (int)p.gd.d) return;
+    float mm = -INFINITY;
+    for (int i = threadIdx.x; i < jt.n; i += 128) mm = fmaxf(mm, p.part_ml[(jt.slot(i) * TR + r) * 2]);
+    for (int x = 16; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = mm;
+    __syncthreads();
+    mm = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float ref = mm == -INFINITY ? 0.0f : mm;
+    const int g = threadIdx.x / COLS, col = threadIdx.x % COLS;
+    float ll = 0.0f;
+    float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+    for (int i = g; i < jt.n; i += GROUPS) {
+        const size_t at = jt.slot(i) * TR + r;
+        const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + at * 2);
+        const float4 v = *reinterpret_cast<const float4 *>(p.part_o + at * DP + col * 4);
+        const float w = ex2(ml.x - ref);
+        ll += w * ml.y;
+        o.x += w * v.x;
+        o.y += w * v.y;
+        o.z += w * v.z;
+        o.w += w * v.w;
+    }
+    sum[g][col] = o;
+    if (col == 0) lsum[g] = ll;
+    __syncthreads();
+    if (g) return;
+    for (int i = 1; i < GROUPS; ++i) {
+        const float4 v = sum[i][col];
+        ll += lsum[i];
+        o.x += v.x;
+        o.y += v.y;
+        o.z += v.z;
+        o.w += v.w;
+    }
+    const bool some = ll > 0.0f || ll != ll;
+    const float inv = some ? 1.0f / ll : 0.0f;
+    const uint32_t tok = p.gd.div((uint32_t)row);
+    const uint32_t head = jt.at.h * p.gd.d + (row - tok * p.gd.d);
+    if (col * 4 < (int)p.head_dim) {
+        const uint64_t e = (uint64_t)(q.q0 + tok) * p.out_stride + (uint64_t)head * p.head_dim + col * 4;
+        if (p.io_type == T_F32)
+            *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + e) =
+                make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        else
+            *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + e) =
+                make_uint2(pack2(p.io_type, o.x * inv, o.y * inv), pack2(p.io_type, o.z * inv, o.w * inv));
+    }
+    if (p.lse && col == 0)
+        p.lse[(uint64_t)(q.q0 + tok) * (p.n_kv * p.gd.d) + head] = some ? (mm + log2f(ll)) * LN2 : -INFINITY;
 }
 
 template <int TYPE, int DP, int TERMS>
@@ -419,7 +487,7 @@ int launch(AttnParams p, cudaStream_t s) {
     const uint32_t grid = SMS * F::CTAS;
     p.part_ml = p.part_o + (size_t)grid * 2 * TR * DP;
     cudaError_t e = launch_pdl(k_attn_few<TYPE, DP, TERMS>, dim3(grid), dim3(WARPS * 32), F::SMEM, s, p);
-    if (e == cudaSuccess) e = launch_pdl(k_attn_join<S, TR, DP>, dim3(grid - 1, 1), dim3(128), 0, s, p, (int)grid);
+    if (e == cudaSuccess) e = launch_pdl(k_attn_join_few<DP>, dim3(grid - 1, TR), dim3(128), 0, s, p);
     return (int)e;
 }
 template <int TYPE, int DP>

@@ -85,7 +85,7 @@ struct Sched {
 
     struct Shared {
         long long warp_sum[32];
-        long long total, before;
+        long long before;
         Pos pos;
         Geo geo;
     };
@@ -170,37 +170,83 @@ struct Sched {
         return true;
     }
 
-    // A walk over consecutive units.
-    struct Cursor {
+    // A walk over a CTA's consecutive units, item by item: units c0 .. c1 - 1 of the item are the CTA's.
+    struct Items {
         Pos at;
         Req q;
         Geo g;
-        int nt;
-        CK_DEV void set(const AttnParams &p, const Pos &pos, const Geo &geo) {
+        int nt, left, c0, c1;
+        CK_DEV void set(const AttnParams &p, const Pos &pos, const Geo &geo, int n) {
             at = pos;
             g = geo;
             q = load_req(p, pos.r);
             nt = tiles(p, q);
+            left = n;
+            span();
         }
-        CK_DEV bool item_end() const { return at.c == g.nch - 1; }
-        // the next unit; the caller knows that there is one
-        CK_DEV void next(const AttnParams &p) {
-            if (++at.c < g.nch) return;
+        CK_DEV void span() {
+            c0 = at.c;
+            c1 = min(g.nch, c0 + left);
+        }
+        CK_DEV bool whole() const { return c0 == 0 && c1 == g.nch; }
+        // the next item; false at the end of the CTA's range
+        CK_DEV bool next(const AttnParams &p) {
+            left -= c1 - c0;
+            if (left <= 0) return false;
             at.c = 0;
-            if (++at.h < (int)p.n_kv) return;
-            at.h = 0;
-            if (++at.t >= nt) {
-                at.t = 0;
-                do {
-                    if (++at.r >= (int)p.nreq) return;
-                    q = load_req(p, at.r);
-                    nt = tiles(p, q);
-                } while (nt == 0);
+            if (++at.h >= (int)p.n_kv) {
+                at.h = 0;
+                if (++at.t >= nt) {
+                    at.t = 0;
+                    do {
+                        if (++at.r >= (int)p.nreq) return false;
+                        q = load_req(p, at.r);
+                        nt = tiles(p, q);
+                    } while (nt == 0);
+                }
+                g = tile_geo<TR, KC>(p, q, at.t);
             }
-            g = tile_geo<TR, KC>(p, q, at.t);
+            span();
+            return true;
         }
     };
+
+    // What the joining kernel needs of each CTA's start, left in the workspace by the CTA.
+    static CK_DEV void leave_cut(const AttnParams &p, long long U, int C, const Pos &at, const Geo &g) {
+        if (threadIdx.x == 0) {
+            if (blockIdx.x == 0) {
+                p.cuts->units = U;
+                p.cuts->ctas = C;
+            }
+            if ((int)blockIdx.x < C) p.cuts->at[blockIdx.x] = make_int4(at.r, at.t, at.h, at.c);
+            if ((int)blockIdx.x < C) p.cuts->chunks[blockIdx.x] = g.nch;
+        }
+    }
 };
+
+// An item that spans CTAs, seen from boundary j (the start of CTA j's units): found at its first cut only.
+// Its parts are those of CTAs first .. first + n - 1, in each CTA's slot 0 except, where the item does not open
+// the first CTA's range, slot 1 there.
+struct Joint {
+    Pos at;
+    int first, n, slot0;
+    CK_DEV size_t slot(int i) const { return (size_t)(first + i) * 2 + (i == 0 ? slot0 : 0); }
+};
+CK_DEV bool find_joint(const AttnParams &p, int j, Joint &o) {
+    const long long U = p.cuts->units;
+    const int C = p.cuts->ctas;
+    if (j >= C) return false;
+    const int4 v = p.cuts->at[j];
+    const long long u = U * j / C, a = u - v.w, b = a + p.cuts->chunks[j];
+    const long long before = U * (j - 1) / C;
+    if (v.w == 0 || before > a) return false;  // the cut is an item's start, or not its first
+    o.at = {v.x, v.y, v.z, v.w};
+    o.first = j - 1;
+    o.slot0 = before == a ? 0 : 1;
+    // the CTA of unit b - 1: the largest c with U c / C <= b - 1, that is c <= (C b - 1) / U
+    o.n = (int)(((long long)C * b - 1) / U) - o.first + 1;
+    return true;
+}
 
 // The keys that row's token may see: [lo, hi).
 CK_DEV void row_limits(const AttnParams &p, const Req &q, int row, int &lo, int &hi) {
@@ -227,7 +273,7 @@ CK_DEV float value16(uint16_t b, int type) {
 // Where some rows of a tile see a key and others do not, the matrix product takes V's infinities and
 // NaNs as zeros (0 x inf would reach the rows that do not see them); this is what they add to the
 // rows that do: the sum of the non-finite V[j][d] over the visible j of [j0, j1).
-CK_DEV float nonfinite_v(const AttnParams &p, int r, int h, int d, int j0, int j1, int lo, int hi) {
+static __device__ __noinline__ float nonfinite_v(const AttnParams &p, int r, int h, int d, int j0, int j1, int lo, int hi) {
     float s = 0.0f;
     for (int j = max(j0, lo); j < min(j1, hi); ++j) {
         const int64_t at = key_offset(p, r, j);
@@ -244,66 +290,6 @@ CK_DEV float ex2(float x) {
     return y;
 }
 constexpr float LN2 = 0.69314718055994531f;
-
-// Joins the partial results of the items that span CTAs.  Block (j, y) takes the item that boundary
-// j + 1 (the start of CTA j + 1's range) cuts, if it is the item's first cut, and every gridDim.y-th
-// row of its tile.
-template <class S, int TR, int DP>
-__global__ void __launch_bounds__(128) k_attn_join(const AttnParams p, int grid) {
-    __shared__ typename S::Shared sh;
-    grid_dep_trigger_small();
-    grid_dep_wait();
-    long long U;
-    int C;
-    Pos at;
-    Geo g;
-    const int j = (int)blockIdx.x + 1;
-    if (!S::find(p, sh, grid, j, U, C, at, g)) return;
-    const long long u = S::start(U, C, j), a = u - at.c, b = a + g.nch;
-    if (at.c == 0 || S::start(U, C, j - 1) > a) return;  // the cut is an item's start, or not its first
-    const Req q = load_req(p, at.r);
-    const int rows = q.nq * (int)p.gd.d;
-    // CTAs c0 = j - 1 .. c1 hold parts: c0's in its first slot if the item starts its range
-    const int s0 = S::start(U, C, j - 1) == a ? 0 : 1;
-    const auto slot = [&](int c) { return (size_t)c * 2 + (c == j - 1 ? s0 : 0); };
-    const auto holds = [&](int c) { return c < C && S::start(U, C, c) < b; };
-    const int groups = blockDim.x / (DP / 4);  // a thread owns four neighbouring columns of a row
-    const int col = (threadIdx.x % (DP / 4)) * 4;
-    for (int r = (int)blockIdx.y * groups + threadIdx.x / (DP / 4); r < TR; r += gridDim.y * groups) {
-        const int row = at.t * TR + r;
-        if (row >= rows) break;
-        float mm = -INFINITY;
-        for (int c = j - 1; holds(c); ++c) mm = fmaxf(mm, p.part_ml[(slot(c) * TR + r) * 2]);
-        const float ref = mm == -INFINITY ? 0.0f : mm;
-        float ll = 0.0f;
-        float4 o = make_float4(0, 0, 0, 0);
-        for (int c = j - 1; holds(c); ++c) {
-            const float *ml = p.part_ml + (slot(c) * TR + r) * 2;
-            const float w = ex2(ml[0] - ref);
-            const float4 v = *reinterpret_cast<const float4 *>(p.part_o + (slot(c) * TR + r) * DP + col);
-            ll += w * ml[1];
-            o.x += w * v.x;
-            o.y += w * v.y;
-            o.z += w * v.z;
-            o.w += w * v.w;
-        }
-        const bool some = ll > 0.0f || ll != ll;
-        const float inv = some ? 1.0f / ll : 0.0f;
-        const uint32_t tok = p.gd.div((uint32_t)row);
-        const uint32_t head = at.h * p.gd.d + (row - tok * p.gd.d);
-        if (col < (int)p.head_dim) {
-            const uint64_t e = (uint64_t)(q.q0 + tok) * p.out_stride + (uint64_t)head * p.head_dim + col;
-            if (p.io_type == T_F32)
-                *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + e) =
-                    make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-            else
-                *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + e) =
-                    make_uint2(pack2(p.io_type, o.x * inv, o.y * inv), pack2(p.io_type, o.z * inv, o.w * inv));
-        }
-        if (p.lse && col == 0)
-            p.lse[(uint64_t)(q.q0 + tok) * (p.n_kv * p.gd.d) + head] = some ? (mm + log2f(ll)) * LN2 : -INFINITY;
-    }
-}
 
 }  // namespace attn
 }  // namespace ck

@@ -199,12 +199,20 @@ struct KvAppendParams {
 int launch_kv_append(const KvAppendParams &p, int in_type, cudaStream_t s);
 
 // attention over the paged cache (attn_paged.cu, attn_chunk.cu)
+constexpr int ATTN_MAX_CTAS = 148 * 3;
+struct AttnCuts {  // where each CTA's units begin, for the kernel that joins partial results
+    long long units;
+    int ctas, pad;
+    int4 at[ATTN_MAX_CTAS];      // request, tile, head, key chunk
+    int chunks[ATTN_MAX_CTAS];   // key chunks of that item
+};
 struct AttnParams {
     const void *q, *k, *v;
     void *out;
     float *lse;
     const int32_t *table, *kv_len, *q_start;
     float *part_o, *part_ml;  // partial results of work items that span CTAs
+    AttnCuts *cuts;
     int *err;                 // device error word (bounded waits)
     uint64_t q_stride, out_stride, table_stride, block_stride, token_stride, head_stride;
     uint32_t nreq, ntok, n_kv, head_dim, max_blocks, n_blocks;
