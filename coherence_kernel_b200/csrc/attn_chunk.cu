@@ -44,7 +44,7 @@ struct Chunk {
 };
 // mbarriers
 struct Bars {
-    uint64_t full[4], empty[4], q_full, q_empty, s_full[2], p_full[2], o_full[2], done;
+    uint64_t full[4], empty[4], q_full, q_empty, s_full[2], p_half[2], p_full[2], o_full[2], done;
 };
 // tensor memory: scores (and P over them) of the two halves, then their outputs
 CK_DEV uint32_t s_col(int t) { return (uint32_t)t * 128; }
@@ -159,6 +159,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) k_attn_chunk(const __grid_constan
         mbar_init(&bar->q_empty, 1);
         for (int t = 0; t < 2; ++t) {
             mbar_init(&bar->s_full[t], 1);
+            mbar_init(&bar->p_half[t], 128);
             mbar_init(&bar->p_full[t], 128);
             mbar_init(&bar->o_full[t], 1);
         }
@@ -199,60 +200,33 @@ __global__ void __launch_bounds__(NTHREADS, 1) k_attn_chunk(const __grid_constan
                      static_cast<const uint16_t *>(base) + (live ? o + c * 8 : 0), live);
             }
         };
-        // copies not yet handed over, oldest first: at most two groups stay in flight behind the newest
-        uint64_t *pend[3] = {nullptr, nullptr, nullptr};
-        int npend = 0;
-        uint32_t clean[3] = {0, 0, 0};  // a V tile to clear of infinities and NaNs first: its address, else 0
-        uint32_t clean_item[3] = {0, 0, 0};
-        const auto hand_over = [&]() {  // the oldest: its copies have landed
-            if (clean[0]) {
-                bool bad = false;
-                for (int i = 0; i < PIECES; ++i) {
-                    const int row = w * 32 + i * ROWS_PER + lane / PIECES, c = lane % PIECES;
-                    const uint32_t a = clean[0] - sbase + (c >> 3) * (F::TILE / F::HALVES) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
-                    uint4 *v = reinterpret_cast<uint4 *>(smem + a);
-                    uint4 x = *v;
-                    bool b = false;
-                    x.x = finite2<TYPE>(x.x, b);
-                    x.y = finite2<TYPE>(x.y, b);
-                    x.z = finite2<TYPE>(x.z, b);
-                    x.w = finite2<TYPE>(x.w, b);
-                    if (b) *v = x;
-                    bad |= b;
-                }
-                if (bad) poison[(clean_item[0] - 1) & 7] = clean_item[0];
-            }
-            fence_proxy_async_smem();
-            mbar_arrive(pend[0]);
-            pend[0] = pend[1];
-            pend[1] = pend[2];
-            clean[0] = clean[1];
-            clean[1] = clean[2];
-            clean_item[0] = clean_item[1];
-            clean_item[1] = clean_item[2];
-            --npend;
+        // The copies arrive on the barrier themselves once they have landed, so the loader runs as far ahead as
+        // the ring lets it; the thread that issues the products runs the proxy fence after its wait.
+        const auto hand_over = [&](uint64_t *b) {
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(b)) : "memory");
         };
-        const auto push = [&](uint64_t *b, uint32_t tile_to_clean, uint32_t item) {
+        // A V tile with keys that only some rows see: infinities and NaNs become zeros before it is handed over
+        const auto clean = [&](uint32_t tile, uint32_t item) {
             cp_commit();
-            pend[npend] = b;
-            clean[npend] = tile_to_clean;
-            clean_item[npend] = item;
-            ++npend;
-            if (npend == 3) {
-                cp_wait<2>();
-                hand_over();
-            }
-        };
-        const auto drain = [&]() {
             cp_wait<0>();
-            while (npend) hand_over();
+            bool bad = false;
+            for (int i = 0; i < PIECES; ++i) {
+                const int row = w * 32 + i * ROWS_PER + lane / PIECES, c = lane % PIECES;
+                const uint32_t a = tile - sbase + (c >> 3) * (F::TILE / F::HALVES) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+                uint4 *v = reinterpret_cast<uint4 *>(smem + a);
+                uint4 x = *v;
+                bool b = false;
+                x.x = finite2<TYPE>(x.x, b);
+                x.y = finite2<TYPE>(x.y, b);
+                x.z = finite2<TYPE>(x.z, b);
+                x.w = finite2<TYPE>(x.w, b);
+                if (b) *v = x;
+                bad |= b;
+            }
+            if (bad) poison[item & 7] = item + 1;
         };
-        // waits until a buffer is free; everything loaded is handed over before it blocks
         const auto room = [&](uint64_t *b, uint32_t parity) -> bool {
-            if (__all_sync(0xffffffffu, mbar_test_wait(b, parity))) return true;
-            drain();
-            const bool ok = mbar_wait_bounded(b, parity, p.err, 30);
-            return __all_sync(0xffffffffu, ok);
+            return __all_sync(0xffffffffu, mbar_wait_bounded(b, parity, p.err, 30));
         };
         uint32_t e = 0, item = 0;  // ring entries and items so far
         bool ok = true;
@@ -270,7 +244,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) k_attn_chunk(const __grid_constan
                 ok = room(&bar->empty[st], ((e / NS) & 1) ^ 1);
                 if (!ok) break;
                 copy_rows(tile, w * 32, p.k, off);
-                push(&bar->full[st], 0, 0);
+                hand_over(&bar->full[st]);
                 ++e;
                 if (c == it.c0) {  // the item's query rows
                     ok = room(&bar->q_empty, (item & 1) ^ 1);
@@ -287,7 +261,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) k_attn_chunk(const __grid_constan
                         // rows 0-127 and 128-255 are a tile each
                         copy_rows(sbase + F::Q_OFF + (w >> 1) * F::TILE, (w & 1) * 64 + b * 32, p.q, o);
                     }
-                    push(&bar->q_full, 0, 0);
+                    hand_over(&bar->q_full);
                 }
                 // V
                 st = e % NS;
@@ -295,12 +269,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) k_attn_chunk(const __grid_constan
                 ok = room(&bar->empty[st], ((e / NS) & 1) ^ 1);
                 if (!ok) break;
                 copy_rows(tile, w * 32, p.v, off);
-                push(&bar->full[st], partial ? tile : 0, item + 1);
+                if (partial) clean(tile, item);
+                hand_over(&bar->full[st]);
                 ++e;
             }
             ++item;
         } while (ok && it.next(p));
-        drain();
+        cp_commit();
+        cp_wait<0>();  // no copy outlives the thread, also after a wait gave up
     } else if (wg == 3) {
         // ---------------------------------------------------------------------------- the products
         reg_dec<64>();
@@ -318,9 +294,17 @@ __global__ void __launch_bounds__(NTHREADS, 1) k_attn_chunk(const __grid_constan
             };
             const auto wait = [&](uint64_t *b, uint32_t parity, int code) -> bool {
                 const bool ok = mbar_wait_bounded(b, parity, p.err, code);
-                const bool all = __all_sync(0xffffffffu, ok);
+                return __all_sync(0xffffffffu, ok);
+            };
+            const auto wait_tile = [&](uint64_t *b, uint32_t parity, int code) -> bool {
+                const bool ok = wait(b, parity, code);
+                fence_proxy_async_smem();  // the loader's writes, before the tensor core reads them
+                return ok;
+            };
+            const auto wait_weights = [&](uint64_t *b, uint32_t parity, int code) -> bool {
+                const bool ok = wait(b, parity, code);
                 tc_fence_after();
-                return all;
+                return ok;
             };
             // S_t = Q_t K^T from ring stage st; free: barriers of what this was the last use of
             const auto scores = [&](int t, uint32_t st, bool k_done, bool q_done) {
@@ -337,13 +321,15 @@ __global__ void __launch_bounds__(NTHREADS, 1) k_attn_chunk(const __grid_constan
                 }
                 __syncwarp();
             };
-            // O_t (+)= P_t V from ring stage st
-            const auto values = [&](int t, uint32_t st, bool first, bool v_done, bool o_done) {
+            // O_t (+)= P_t V over half h of the unit's keys, from ring stage st
+            const auto values = [&](int t, int h, uint32_t st, bool first, bool v_done, bool o_done) {
                 const uint64_t vd = v_desc + st * STAGE16;
                 if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < KC / 16; ++k)
-                        umma_bf16_ts(tmem + o_col(t), tmem + s_col(t) + k * 8, vd + k * 128, id_o, !(first && k == 0));
+                    for (int k = 0; k < KC / 32; ++k) {
+                        const int kk = h * (KC / 32) + k;
+                        umma_bf16_ts(tmem + o_col(t), tmem + s_col(t) + kk * 8, vd + kk * 128, id_o, !(first && kk == 0));
+                    }
                     if (v_done) umma_commit(&bar->empty[st]);
                     if (o_done) umma_commit(&bar->o_full[t]);
                 }
@@ -353,21 +339,24 @@ __global__ void __launch_bounds__(NTHREADS, 1) k_attn_chunk(const __grid_constan
             bool ok = true;
             do {
                 const int nh = halves(p, it.q, it.at.t), units = it.c1 - it.c0;
-                ok = wait(&bar->q_full, item & 1, 31) && wait(&bar->full[e % NS], (e / NS) & 1, 32);
+                ok = wait_tile(&bar->q_full, item & 1, 31) && wait_tile(&bar->full[e % NS], (e / NS) & 1, 32);
                 if (!ok) break;
                 for (int t = 0; t < nh; ++t) scores(t, e % NS, t == nh - 1, t == nh - 1 && units == 1);
                 ++e;
                 for (int c = 0; c < units && ok; ++c) {
                     const bool last = c == units - 1;
                     const uint32_t sv = e % NS, sk = (e + 1) % NS;
-                    ok = wait(&bar->full[sv], (e / NS) & 1, 33);
+                    ok = wait_tile(&bar->full[sv], (e / NS) & 1, 33);
                     for (int t = 0; t < nh && ok; ++t) {
-                        ok = wait(&bar->p_full[t], handed[t] & 1, 34);
+                        ok = wait_weights(&bar->p_half[t], handed[t] & 1, 34);
+                        if (!ok) break;
+                        values(t, 0, sv, c == 0, false, false);
+                        ok = wait_weights(&bar->p_full[t], handed[t] & 1, 36);
                         if (!ok) break;
                         ++handed[t];
-                        values(t, sv, c == 0, t == nh - 1, last);
+                        values(t, 1, sv, c == 0, t == nh - 1, last);
                         if (!last) {
-                            if (t == 0) ok = wait(&bar->full[sk], ((e + 1) / NS) & 1, 35);
+                            if (t == 0) ok = wait_tile(&bar->full[sk], ((e + 1) / NS) & 1, 35);
                             if (ok) scores(t, sk, t == nh - 1, t == nh - 1 && c == units - 2);
                         }
                     }
@@ -473,6 +462,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) k_attn_chunk(const __grid_constan
                         pk[x] = pack2(TYPE, v.x, v.y);
                     }
                     tmem_st16(s_at + b * 16, pk);
+                    if (b == 1) {  // the first half of the keys: its product can start
+                        tmem_st_wait();
+                        tc_fence_before();
+                        mbar_arrive(&bar->p_half[t]);
+                    }
                 }
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 tmem_st_wait();
