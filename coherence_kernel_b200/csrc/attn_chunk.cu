@@ -44,7 +44,7 @@ struct Chunk {
 };
 // mbarriers
 struct Bars {
-    uint64_t full[4], empty[4], q_full, q_empty, s_full[2], p_half[2], p_full[2], o_full[2], done;
+    uint64_t full[4], empty[4], raw[4], q_full, q_empty, s_full[2], p_half[2], p_full[2], o_full[2], done;
 };
 // tensor memory: scores (and P over them) of the two halves, then their outputs
 CK_DEV uint32_t s_col(int t) { return (uint32_t)t * 128; }
@@ -125,8 +125,10 @@ __device__ __noinline__ void add_nonfinite(const AttnParams &p, const Pos &at, c
     }
 }
 
-template <int TYPE, int DP>
-__global__ void __launch_bounds__(NTHREADS, 1) k_attn_chunk(const __grid_constant__ AttnParams p) {
+template <int TYPE, int DP, bool TMA>
+__global__ void __launch_bounds__(NTHREADS, 1)
+    k_attn_chunk(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap kmap,
+                 const __grid_constant__ CUtensorMap vmap, int box) {
     using F = Chunk<DP>;
     constexpr int PIECES = DP / 8;           // 16-byte pieces of a row
     constexpr int ROWS_PER = 32 / PIECES;    // rows one warp instruction copies
@@ -152,10 +154,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) k_attn_chunk(const __grid_constan
     const int n = (int)(S::start(U, C, blockIdx.x + 1) - S::start(U, C, blockIdx.x));
     if (threadIdx.x == 0) {
         for (int i = 0; i < NS; ++i) {
-            mbar_init(&bar->full[i], 128);
+            mbar_init(&bar->full[i], TMA ? 1 : 128);
             mbar_init(&bar->empty[i], 1);
+            mbar_init(&bar->raw[i], 1);
         }
-        mbar_init(&bar->q_full, 128);
+        mbar_init(&bar->q_full, TMA ? 96 : 128);
         mbar_init(&bar->q_empty, 1);
         for (int t = 0; t < 2; ++t) {
             mbar_init(&bar->s_full[t], 1);
@@ -180,23 +183,20 @@ __global__ void __launch_bounds__(NTHREADS, 1) k_attn_chunk(const __grid_constan
         // -------------------------------------------------------------------------------- loader
         reg_dec<80>();
         const int w = warp - 8;
+        constexpr uint32_t HALF = F::TILE / F::HALVES;
         typename S::Items it;
         it.set(p, pos, geo, n);
-        // lane l holds key 32 w + l of unit c: its element offset, -1 to fill with zeros
-        const auto lookup = [&](int c) -> int64_t {
-            const int j = it.g.lo + c * KC + w * 32 + lane;
-            if (j >= it.g.hi) return -1;
-            const int64_t o = key_offset(p, it.at.r, j);
-            return o < 0 ? -1 : o + (int64_t)(it.at.h * p.head_stride);
+        const auto room = [&](uint64_t *b, uint32_t parity) -> bool {
+            return __all_sync(0xffffffffu, mbar_wait_bounded(b, parity, p.err, 30));
         };
-        // 32 rows of a tile by this warp
+        // 32 rows of a tile by one warp: lane l has the element offset of row l, -1 to fill it with zeros
         const auto copy_rows = [&](uint32_t tile, int row0, const void *base, int64_t off) {
 #pragma unroll 4
             for (int i = 0; i < PIECES; ++i) {
                 const int lr = i * ROWS_PER + lane / PIECES, c = lane % PIECES, row = row0 + lr;
                 const int64_t o = __shfl_sync(0xffffffffu, off, lr);
                 const bool live = o >= 0 && c * 8 < (int)p.head_dim;
-                cp16(tile + (c >> 3) * (F::TILE / F::HALVES) + row * 128 + (((c & 7) ^ (row & 7)) << 4),
+                cp16(tile + (c >> 3) * HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4),
                      static_cast<const uint16_t *>(base) + (live ? o + c * 8 : 0), live);
             }
         };
@@ -205,15 +205,29 @@ __global__ void __launch_bounds__(NTHREADS, 1) k_attn_chunk(const __grid_constan
         const auto hand_over = [&](uint64_t *b) {
             asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(b)) : "memory");
         };
-        // A V tile with keys that only some rows see: infinities and NaNs become zeros before it is handed over
-        const auto clean = [&](uint32_t tile, uint32_t item) {
-            cp_commit();
-            cp_wait<0>();
+        // query rows 32 b .. 32 b + 31 of the item; rows 0-127 and 128-255 are a tile each
+        const auto copy_queries = [&](int b) {
+            const int row = it.at.t * TR + b * 32 + lane;
+            int64_t o = -1;
+            if (row < it.q.nq * (int)p.gd.d) {
+                const uint32_t tok = p.gd.div((uint32_t)row);
+                o = (int64_t)((uint64_t)(it.q.q0 + tok) * p.q_stride +
+                              (uint64_t)(it.at.h * p.gd.d + row - tok * p.gd.d) * p.head_dim);
+            }
+            copy_rows(sbase + F::Q_OFF + (b >> 2) * F::TILE, (b & 3) * 32, p.q, o);
+        };
+        // The first rows of a V tile with keys that only some rows see, `step` threads together: infinities and NaNs
+        // become zeros, and so do the rows of keys past the last (n_keys on), which hold whatever the page does.
+        const auto clean = [&](uint32_t tile, uint32_t item, int rows, int first, int step, int n_keys) {
             bool bad = false;
-            for (int i = 0; i < PIECES; ++i) {
-                const int row = w * 32 + i * ROWS_PER + lane / PIECES, c = lane % PIECES;
-                const uint32_t a = tile - sbase + (c >> 3) * (F::TILE / F::HALVES) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+            for (int i = first; i < rows * PIECES; i += step) {
+                const int row = i / PIECES, c = i % PIECES;
+                const uint32_t a = tile - sbase + (c >> 3) * HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4);
                 uint4 *v = reinterpret_cast<uint4 *>(smem + a);
+                if (row >= n_keys) {
+                    *v = make_uint4(0, 0, 0, 0);
+                    continue;
+                }
                 uint4 x = *v;
                 bool b = false;
                 x.x = finite2<TYPE>(x.x, b);
@@ -225,56 +239,123 @@ __global__ void __launch_bounds__(NTHREADS, 1) k_attn_chunk(const __grid_constan
             }
             if (bad) poison[item & 7] = item + 1;
         };
-        const auto room = [&](uint64_t *b, uint32_t parity) -> bool {
-            return __all_sync(0xffffffffu, mbar_wait_bounded(b, parity, p.err, 30));
-        };
         uint32_t e = 0, item = 0;  // ring entries and items so far
         bool ok = true;
-        do {
-            int all_lo, all_hi;
-            item_limits(p, it.q, it.at.t, all_lo, all_hi);
-            int64_t next = lookup(it.c0);
-            for (int c = it.c0; c < it.c1 && ok; ++c) {
-                const int64_t off = next;
-                if (c + 1 < it.c1) next = lookup(c + 1);
-                const int j0 = it.g.lo + c * KC;
-                const bool partial = j0 < all_lo || j0 + KC > all_hi;
-                // K
-                uint32_t st = e % NS, tile = sbase + F::RING_OFF + st * F::TILE;
-                ok = room(&bar->empty[st], ((e / NS) & 1) ^ 1);
-                if (!ok) break;
-                copy_rows(tile, w * 32, p.k, off);
-                hand_over(&bar->full[st]);
-                ++e;
-                if (c == it.c0) {  // the item's query rows
+        if constexpr (TMA) {
+            if (w == 0) {
+                // K and V: a lane per box of the unit looks its page up a unit ahead and issues its loads
+                const int boxes = KC / box;
+                uint32_t to_raw = 0;  // a bit per stage: its last loads went to the raw barrier
+                uint32_t raw_phase = 0;
+                const auto lookup = [&](int c) -> int2 {  // page (past the last: zeros) and token of the lane's box
+                    const int j = it.g.lo + c * KC + lane * box;
+                    if (lane >= boxes || j >= it.g.hi) return make_int2((int)p.n_blocks, 0);
+                    const uint32_t b = p.btd.div((uint32_t)j);
+                    const int pg = p.table[(uint64_t)it.at.r * p.table_stride + b];
+                    return make_int2(pg >= 0 && pg < (int)p.n_blocks ? pg : (int)p.n_blocks, j - (int)(b * p.btd.d));
+                };
+                do {
+                    int all_lo, all_hi;
+                    item_limits(p, it.q, it.at.t, all_lo, all_hi);
+                    int2 next = lookup(it.c0);
+                    for (int c = it.c0; c < it.c1 && ok; ++c) {
+                        const int2 at = next;
+                        if (c + 1 < it.c1) next = lookup(c + 1);
+                        const int j0 = it.g.lo + c * KC;
+                        const bool partial = j0 < all_lo || j0 + KC > all_hi;
+                        for (int kv = 0; kv < 2; ++kv, ++e) {
+                            const uint32_t st = e % NS, tile = sbase + F::RING_OFF + st * F::TILE + lane * box * 128;
+                            ok = room(&bar->empty[st], ((e / NS) & 1) ^ 1);
+                            if (!ok) break;
+                            const bool raw = kv && partial;
+                            uint64_t *full = raw ? &bar->raw[st] : &bar->full[st];
+                            to_raw = (to_raw & ~(1u << st)) | (uint32_t)raw << st;
+                            raw_phase ^= (uint32_t)raw << st;  // after it: the parity of the next use
+                            if (lane == 0) mbar_arrive_expect_tx(full, F::TILE);
+                            __syncwarp();
+                            if (lane < boxes) {
+                                const CUtensorMap *map = kv ? &vmap : &kmap;
+#pragma unroll
+                                for (int x = 0; x < F::HALVES; ++x)
+                                    tma_load_kv(tile + x * HALF, map, full, x * 64, it.at.h, at.y, at.x);
+                            }
+                            __syncwarp();
+                        }
+                    }
+                } while (ok && it.next(p));
+                // after a wait gave up, no load outlives the block
+                for (uint32_t x = e > NS ? e - NS : 0; !ok && x < e; ++x) {
+                    const uint32_t st = x % NS;
+                    if (to_raw >> st & 1) mbar_wait_bounded(&bar->raw[st], (raw_phase >> st & 1) ^ 1, nullptr, 0);
+                    else mbar_wait_bounded(&bar->full[st], (x / NS) & 1, nullptr, 0);
+                }
+            } else {
+                // the queries, and the V tiles to clean
+                const int me = threadIdx.x - 288;  // 0 .. 95
+                uint32_t raw_parity = 0;           // a bit per stage
+                do {
                     ok = room(&bar->q_empty, (item & 1) ^ 1);
                     if (!ok) break;
-                    const int rows = it.q.nq * (int)p.gd.d;
-                    for (int b = 0; b < 2; ++b) {
-                        const int row = it.at.t * TR + w * 64 + b * 32 + lane;
-                        int64_t o = -1;
-                        if (row < rows) {
-                            const uint32_t tok = p.gd.div((uint32_t)row);
-                            o = (int64_t)((uint64_t)(it.q.q0 + tok) * p.q_stride +
-                                          (uint64_t)(it.at.h * p.gd.d + row - tok * p.gd.d) * p.head_dim);
-                        }
-                        // rows 0-127 and 128-255 are a tile each
-                        copy_rows(sbase + F::Q_OFF + (w >> 1) * F::TILE, (w & 1) * 64 + b * 32, p.q, o);
-                    }
+                    for (int b = w - 1; b < TR / 32; b += 3) copy_queries(b);
                     hand_over(&bar->q_full);
-                }
-                // V
-                st = e % NS;
-                tile = sbase + F::RING_OFF + st * F::TILE;
-                ok = room(&bar->empty[st], ((e / NS) & 1) ^ 1);
-                if (!ok) break;
-                copy_rows(tile, w * 32, p.v, off);
-                if (partial) clean(tile, item);
-                hand_over(&bar->full[st]);
-                ++e;
+                    int all_lo, all_hi;
+                    item_limits(p, it.q, it.at.t, all_lo, all_hi);
+                    for (int c = it.c0; c < it.c1 && ok; ++c, e += 2) {
+                        const int j0 = it.g.lo + c * KC;
+                        if (j0 >= all_lo && j0 + KC <= all_hi) continue;
+                        const uint32_t st = (e + 1) % NS;
+                        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&bar->raw[st], raw_parity >> st & 1, p.err, 41));
+                        if (!ok) break;
+                        raw_parity ^= 1u << st;
+                        clean(sbase + F::RING_OFF + st * F::TILE, item, KC, me, 96, it.g.hi - j0);
+                        fence_proxy_async_smem();
+                        asm volatile("bar.sync 1, 96;" ::: "memory");
+                        if (me == 0) mbar_arrive(&bar->full[st]);
+                    }
+                    ++item;
+                } while (ok && it.next(p));
             }
-            ++item;
-        } while (ok && it.next(p));
+        } else {
+            // pages of other sizes: 16-byte copies, lane l of warp w looks up key 32 w + l a unit ahead
+            const auto lookup = [&](int c) -> int64_t {
+                const int j = it.g.lo + c * KC + w * 32 + lane;
+                if (j >= it.g.hi) return -1;
+                const int64_t o = key_offset(p, it.at.r, j);
+                return o < 0 ? -1 : o + (int64_t)(it.at.h * p.head_stride);
+            };
+            do {
+                int all_lo, all_hi;
+                item_limits(p, it.q, it.at.t, all_lo, all_hi);
+                int64_t next = lookup(it.c0);
+                for (int c = it.c0; c < it.c1 && ok; ++c) {
+                    const int64_t off = next;
+                    if (c + 1 < it.c1) next = lookup(c + 1);
+                    const int j0 = it.g.lo + c * KC;
+                    const bool partial = j0 < all_lo || j0 + KC > all_hi;
+                    for (int kv = 0; kv < 2; ++kv, ++e) {
+                        const uint32_t st = e % NS, tile = sbase + F::RING_OFF + st * F::TILE;
+                        ok = room(&bar->empty[st], ((e / NS) & 1) ^ 1);
+                        if (!ok) break;
+                        copy_rows(tile, w * 32, kv ? p.v : p.k, off);
+                        if (kv && partial) {
+                            cp_commit();
+                            cp_wait<0>();
+                            __syncwarp();  // a warp cleans the rows it copied
+                            clean(tile + w * 32 * 128, item, 32, lane, 32, 32);
+                        }
+                        hand_over(&bar->full[st]);
+                        if (kv == 0 && c == it.c0) {  // the item's queries
+                            ok = room(&bar->q_empty, (item & 1) ^ 1);
+                            if (!ok) break;
+                            copy_queries(2 * w);
+                            copy_queries(2 * w + 1);
+                            hand_over(&bar->q_full);
+                        }
+                    }
+                }
+                ++item;
+            } while (ok && it.next(p));
+        }
         cp_commit();
         cp_wait<0>();  // no copy outlives the thread, also after a wait gave up
     } else if (wg == 3) {
@@ -565,20 +646,32 @@ __global__ void __launch_bounds__(TR) k_attn_join_chunk(const __grid_constant__ 
         p.lse[(uint64_t)(q.q0 + tok) * (p.n_kv * p.gd.d) + head] = some ? (mm + log2f(ll)) * LN2 : -INFINITY;
 }
 
-template <int TYPE, int DP>
-int launch(AttnParams p, cudaStream_t s) {
+template <int TYPE, int DP, bool TMA>
+int launch(AttnParams p, int box, cudaStream_t s) {
     using F = Chunk<DP>;
     static unsigned long long done = 0;
     if (attr_pending(done)) {
-        cudaError_t e = cudaFuncSetAttribute(k_attn_chunk<TYPE, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM);
+        cudaError_t e = cudaFuncSetAttribute(k_attn_chunk<TYPE, DP, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM);
         if (e != cudaSuccess) return (int)e;
         attr_mark(done);
     }
     const uint32_t grid = SMS;
     p.part_ml = p.part_o + (size_t)grid * 2 * TR * DP;
-    cudaError_t e = launch_pdl(k_attn_chunk<TYPE, DP>, dim3(grid), dim3(NTHREADS), F::SMEM, s, p);
+    CUtensorMap kmap = {}, vmap = {};
+    cudaError_t e;
+    if (TMA && (make_kv_map(&kmap, p.k, p, box) || make_kv_map(&vmap, p.v, p, box))) return CK_ERR_ARG;
+    e = launch_pdl(k_attn_chunk<TYPE, DP, TMA>, dim3(grid), dim3(NTHREADS), F::SMEM, s, p, kmap, vmap, box);
     if (e == cudaSuccess) e = launch_pdl(k_attn_join_chunk<DP>, dim3(grid - 1, DP / 8), dim3(TR), 0, s, p);
     return (int)e;
+}
+
+// TMA where the pages allow it (2048 new tokens of 8192, pages of 16: 16-byte copies keep a loader at 21 bytes per
+// cycle and SM, about 1500 cycles a tile, and bound the kernel), else the copies.
+template <int TYPE, int DP>
+int launch_pages(const AttnParams &p, cudaStream_t s) {
+    const int box = kv_box(p.btd.d, 64);
+    const bool strides = p.token_stride && p.block_stride && p.head_stride;
+    return box && strides ? launch<TYPE, DP, true>(p, box, s) : launch<TYPE, DP, false>(p, 0, s);
 }
 
 }  // namespace
@@ -591,8 +684,8 @@ size_t attn_chunk_workspace_bytes(uint32_t head_dim) {
 int launch_attn_chunk(const AttnParams &p, cudaStream_t s) {
     if (!attn_chunk_ok_types(p.io_type, p.cache_type, p.head_dim)) return CK_ERR_SHAPE;
     if (p.cache_type == T_BF16)
-        return p.head_dim <= 64 ? attn::launch<T_BF16, 64>(p, s) : attn::launch<T_BF16, 128>(p, s);
-    return p.head_dim <= 64 ? attn::launch<T_F16, 64>(p, s) : attn::launch<T_F16, 128>(p, s);
+        return p.head_dim <= 64 ? attn::launch_pages<T_BF16, 64>(p, s) : attn::launch_pages<T_BF16, 128>(p, s);
+    return p.head_dim <= 64 ? attn::launch_pages<T_F16, 64>(p, s) : attn::launch_pages<T_F16, 128>(p, s);
 }
 
 }  // namespace ck

@@ -32,15 +32,16 @@ CK_DEV Req load_req(const AttnParams &p, int r) {
 struct Geo {
     int lo, hi, nch;  // keys [lo, hi) of the tile and its chunks (at least one, so that empty rows are written)
 };
-// Keys a tile of rows [row, row + TR) sees: the last row's upper bound, the first row's lower one.
-template <int TR, int KC>
+// Keys a tile of rows [row, row + TR) sees: the last row's upper bound, the first row's lower one (down to a multiple
+// of ALIGN).
+template <int TR, int KC, int ALIGN>
 CK_DEV Geo tile_geo(const AttnParams &p, const Req &q, int t) {
     const int rows = q.nq * (int)p.gd.d;
     const int first = t * TR, last = min(first + TR, rows) - 1;
     const int base = q.kl - q.nq;  // position of the request's first new token
     Geo g;
     g.hi = p.causal ? min(q.kl, base + (int)p.gd.div(last) + 1) : q.kl;
-    g.lo = p.window ? max(0, base + (int)p.gd.div(first) - p.window + 1) & ~15 : 0;
+    g.lo = p.window ? max(0, base + (int)p.gd.div(first) - p.window + 1) & ~(ALIGN - 1) : 0;
     if (g.hi <= g.lo) {
         g.lo = g.hi = 0;
         g.nch = 1;
@@ -57,6 +58,7 @@ struct Pos {
 // The kind of request a kernel takes: few rows, or many (CHUNK).
 template <int TR, int KC, bool CHUNK>
 struct Sched {
+    static constexpr int ALIGN = CHUNK ? 64 : 16;
     static CK_DEV int tiles(const AttnParams &p, const Req &q) {
         const int rows = q.nq * (int)p.gd.d;
         if (CHUNK ? rows < (int)p.row_split : rows >= (int)p.row_split) return 0;
@@ -69,14 +71,14 @@ struct Sched {
         const int nt = r < (int)p.nreq ? tiles(p, q) : 0;
         long long n = 0;
         if (nt <= 4)
-            for (int t = 0; t < nt; ++t) n += tile_geo<TR, KC>(p, q, t).nch;
+            for (int t = 0; t < nt; ++t) n += tile_geo<TR, KC, ALIGN>(p, q, t).nch;
         // requests of many tiles: the warp's lanes share them out
         for (uint32_t todo = __ballot_sync(0xffffffffu, nt > 4); todo; todo &= todo - 1) {
             const int src = __ffs(todo) - 1;
             const Req w = {0, __shfl_sync(0xffffffffu, q.nq, src), __shfl_sync(0xffffffffu, q.kl, src)};
             const int wt = __shfl_sync(0xffffffffu, nt, src);
             int part = 0;
-            for (int t = threadIdx.x & 31; t < wt; t += 32) part += tile_geo<TR, KC>(p, w, t).nch;
+            for (int t = threadIdx.x & 31; t < wt; t += 32) part += tile_geo<TR, KC, ALIGN>(p, w, t).nch;
             part = __reduce_add_sync(0xffffffffu, part);
             if ((int)(threadIdx.x & 31) == src) n = part;
         }
@@ -143,7 +145,7 @@ struct Sched {
             for (int tb = 0; tb < nt; tb += 32) {
                 const int t = tb + lane;
                 Geo g = {0, 0, 0};
-                if (t < nt) g = tile_geo<TR, KC>(p, q, t);
+                if (t < nt) g = tile_geo<TR, KC, ALIGN>(p, q, t);
                 const long long m = (long long)g.nch * p.n_kv;
                 long long s = m;
                 for (int o = 1; o < 32; o <<= 1) {
@@ -204,7 +206,7 @@ struct Sched {
                         nt = tiles(p, q);
                     } while (nt == 0);
                 }
-                g = tile_geo<TR, KC>(p, q, at.t);
+                g = tile_geo<TR, KC, ALIGN>(p, q, at.t);
             }
             span();
             return true;
@@ -246,6 +248,43 @@ CK_DEV bool find_joint(const AttnParams &p, int j, Joint &o) {
     // the CTA of unit b - 1: the largest c with U c / C <= b - 1, that is c <= (C b - 1) / U
     o.n = (int)(((long long)C * b - 1) / U) - o.first + 1;
     return true;
+}
+
+// TMA loads of a cache: a 4D map (dim, head, token of a page, page), a box of 64 dims (128 bytes, swizzled) of one
+// head for `box` consecutive tokens of one page.  Pages whose token count is a multiple of 8 qualify; a page past
+// the last reads as zeros.
+CK_DEV void tma_load_kv(uint32_t dst, const CUtensorMap *map, uint64_t *bar, int d, int head, int tok, int page) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"((uint64_t)map), "r"(smem_u32(bar)), "r"(d), "r"(head), "r"(tok), "r"(page)
+        : "memory");
+}
+inline int kv_box(uint32_t block_tokens, int most) {
+    int b = most;
+    while (b >= 8 && block_tokens % b) b >>= 1;
+    return b >= 8 ? b : 0;
+}
+inline int make_kv_map(CUtensorMap *m, const void *base, const AttnParams &p, int box) {
+    using Fn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                            const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                            CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Fn enc = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+                       q == cudaDriverEntryPointSuccess
+                   ? reinterpret_cast<Fn>(f)
+                   : nullptr;
+    }();
+    if (!enc) return CK_ERR_NODEV;
+    const cuuint64_t dims[4] = {p.head_dim, p.n_kv, p.btd.d, p.n_blocks};
+    const cuuint64_t strides[3] = {p.head_stride * 2, p.token_stride * 2, p.block_stride * 2};
+    const cuuint32_t box4[4] = {64, 1, (cuuint32_t)box, 1}, one[4] = {1, 1, 1, 1};
+    const CUresult r = enc(m, p.cache_type == T_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                           const_cast<void *>(base), dims, strides, box4, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : CK_ERR_ARG;
 }
 
 // The keys that row's token may see: [lo, hi).
