@@ -111,20 +111,6 @@ CK_DEV float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-// What V's infinities and NaNs, taken as zeros in the units that some row of the item sees in part, add to one
-// row's columns d0 .. d0 + 15.
-__device__ __noinline__ void add_nonfinite(const AttnParams &p, const Pos &at, const Req &q, const Geo &g, int c0, int c1,
-                                           int d0, int lo, int hi, float (&v)[16]) {
-    int all_lo, all_hi;
-    item_limits(p, q, at.t, all_lo, all_hi);
-    for (int c = c0; c < c1; ++c) {
-        const int j = g.lo + c * KC;
-        if (j >= all_lo && j + KC <= all_hi) continue;
-        for (int x = 0; x < 16; ++x)
-            if (d0 + x < (int)p.head_dim) v[x] += nonfinite_v(p, at.r, at.h, d0 + x, j, min(j + KC, g.hi), lo, hi);
-    }
-}
-
 template <int TYPE, int DP, bool TMA>
 __global__ void __launch_bounds__(NTHREADS, 1)
     k_attn_chunk(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap kmap,
@@ -187,7 +173,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         typename S::Items it;
         it.set(p, pos, geo, n);
         const auto room = [&](uint64_t *b, uint32_t parity) -> bool {
-            return __all_sync(0xffffffffu, mbar_wait_bounded(b, parity, p.err, 30));
+            return __all_sync(0xffffffffu, mbar_wait_short(b, parity, p.err, 30));
         };
         // 32 rows of a tile by one warp: lane l has the element offset of row l, -1 to fill it with zeros
         const auto copy_rows = [&](uint32_t tile, int row0, const void *base, int64_t off) {
@@ -286,8 +272,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                 // after a wait gave up, no load outlives the block
                 for (uint32_t x = e > NS ? e - NS : 0; !ok && x < e; ++x) {
                     const uint32_t st = x % NS;
-                    if (to_raw >> st & 1) mbar_wait_bounded(&bar->raw[st], (raw_phase >> st & 1) ^ 1, nullptr, 0);
-                    else mbar_wait_bounded(&bar->full[st], (x / NS) & 1, nullptr, 0);
+                    if (to_raw >> st & 1) mbar_wait_short(&bar->raw[st], (raw_phase >> st & 1) ^ 1, nullptr, 0);
+                    else mbar_wait_short(&bar->full[st], (x / NS) & 1, nullptr, 0);
                 }
             } else {
                 // the queries, and the V tiles to clean
@@ -304,7 +290,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                         const int j0 = it.g.lo + c * KC;
                         if (j0 >= all_lo && j0 + KC <= all_hi) continue;
                         const uint32_t st = (e + 1) % NS;
-                        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&bar->raw[st], raw_parity >> st & 1, p.err, 41));
+                        ok = __all_sync(0xffffffffu, mbar_wait_short(&bar->raw[st], raw_parity >> st & 1, p.err, 41));
                         if (!ok) break;
                         raw_parity ^= 1u << st;
                         clean(sbase + F::RING_OFF + st * F::TILE, item, KC, me, 96, it.g.hi - j0);
@@ -374,7 +360,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                 __syncwarp();
             };
             const auto wait = [&](uint64_t *b, uint32_t parity, int code) -> bool {
-                const bool ok = mbar_wait_bounded(b, parity, p.err, code);
+                const bool ok = mbar_wait_short(b, parity, p.err, code);
                 return __all_sync(0xffffffffu, ok);
             };
             const auto wait_tile = [&](uint64_t *b, uint32_t parity, int code) -> bool {
@@ -447,7 +433,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             } while (ok && it.next(p));
             // every product has completed before tensor memory is freed, also after a wait gave up
             commit(&bar->done);
-            mbar_wait_bounded(&bar->done, 0, nullptr, 0);
+            mbar_wait_short(&bar->done, 0, nullptr, 0);
         }
     } else {
         // -------------------------------------------------------------------------------- softmax
@@ -477,7 +463,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             }
             int j0 = it.g.lo + it.c0 * KC;
             for (int c = it.c0; c < it.c1; ++c, j0 += KC) {
-                ok = mbar_wait_bounded(&bar->s_full[t], taken & 1, p.err, 38);
+                ok = mbar_wait_short(&bar->s_full[t], taken & 1, p.err, 38);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 ++taken;
@@ -555,7 +541,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                 mbar_arrive(&bar->p_full[t]);
             }
             if (!ok) break;
-            ok = mbar_wait_bounded(&bar->o_full[t], joined & 1, p.err, 39);
+            ok = mbar_wait_short(&bar->o_full[t], joined & 1, p.err, 39);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             ++joined;
@@ -579,7 +565,14 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                 float v[16];
 #pragma unroll
                 for (int x = 0; x < 16; ++x) v[x] = __uint_as_float(o[x]) * inv;
-                if (cleaned && live) add_nonfinite(p, it.at, it.q, it.g, it.c0, it.c1, b * 16, lo, hi, v);
+                if (cleaned && live) {
+                    int il, ih;
+                    item_limits(p, it.q, it.at.t, il, ih);
+#pragma unroll
+                    for (int x = 0; x < 16; ++x)
+                        v[x] += nonfinite_v(p, it.at.r, it.at.h, b * 16 + x, it.g.lo + it.c0 * KC,
+                                            min(it.g.lo + it.c1 * KC, it.g.hi), KC, il, ih, lo, hi);
+                }
                 if (!whole) {
 #pragma unroll
                     for (int x = 0; x < 16; ++x) po[(b * 16 + x) * TR] = v[x];

@@ -377,13 +377,10 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         v[e] = osum[r * DP + c * 8 + e] * inv;
-                        if (any_bad) {
-                            // the 16-key steps of this segment whose V was cleaned
-                            const int s0 = use.g.lo + use.c0 * KC, s1 = min(use.g.lo + use.c1 * KC, use.g.hi);
-                            for (int j = s0; j < s1; j += WK)
-                                if (TERMS > 1 || j < all_lo || j + WK > all_hi)
-                                    v[e] += nonfinite_v(p, use.at.r, use.at.h, c * 8 + e, j, min(j + WK, s1), lo, hi);
-                        }
+                        if (any_bad)  // TERMS > 1: every step's V was cleaned
+                            v[e] += nonfinite_v(p, use.at.r, use.at.h, c * 8 + e, use.g.lo + use.c0 * KC,
+                                                min(use.g.lo + use.c1 * KC, use.g.hi), WK, TERMS > 1 ? 0x7fffffff : all_lo,
+                                                all_hi, lo, hi);
                     }
                     if (whole)
                         store8(p.out, (uint64_t)(use.q.q0 + tok) * p.out_stride + (uint64_t)head * p.head_dim + c * 8,

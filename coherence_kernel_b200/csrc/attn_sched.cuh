@@ -311,14 +311,21 @@ CK_DEV float value16(uint16_t b, int type) {
 }
 // Where some rows of a tile see a key and others do not, the matrix product takes V's infinities and
 // NaNs as zeros (0 x inf would reach the rows that do not see them); this is what they add to the
-// rows that do: the sum of the non-finite V[j][d] over the visible j of [j0, j1).
-static __device__ __noinline__ float nonfinite_v(const AttnParams &p, int r, int h, int d, int j0, int j1, int lo, int hi) {
+// rows that do: the sum of the non-finite V[j][d] over the visible j of [j0, j1), in the steps of `step` keys that reach
+// outside [all_lo, all_hi), the keys that every row sees.  Rare, so a call; scalars only, so that it keeps nothing
+// of the caller's in memory.
+static __device__ __noinline__ float nonfinite_v(const AttnParams &p, int r, int h, int d, int j0, int j1, int step,
+                                                 int all_lo, int all_hi, int lo, int hi) {
     float s = 0.0f;
-    for (int j = max(j0, lo); j < min(j1, hi); ++j) {
-        const int64_t at = key_offset(p, r, j);
-        if (at < 0) continue;
-        const uint16_t b = static_cast<const uint16_t *>(p.v)[at + (int64_t)(h * p.head_stride) + d];
-        if (!finite16(b, p.cache_type)) s += value16(b, p.cache_type);
+    if (d >= (int)p.head_dim) return s;
+    for (int b = j0; b < j1; b += step) {
+        if (b >= all_lo && b + step <= all_hi) continue;
+        for (int j = max(b, lo); j < min(min(b + step, j1), hi); ++j) {
+            const int64_t at = key_offset(p, r, j);
+            if (at < 0) continue;
+            const uint16_t w = static_cast<const uint16_t *>(p.v)[at + (int64_t)(h * p.head_stride) + d];
+            if (!finite16(w, p.cache_type)) s += value16(w, p.cache_type);
+        }
     }
     return s;
 }

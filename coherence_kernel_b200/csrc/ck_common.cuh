@@ -114,6 +114,14 @@ CK_DEV bool mbar_wait_bounded_ns(uint64_t *bar, uint32_t parity, int *err, int c
     if (err) atomicCAS(err, 0, code);
     return false;
 }
+// The same for waits that are mostly short: reading the global timer costs several hundred cycles, so it
+// is not read until a few hundred probes (each of which suspends the thread for a while) have failed.
+CK_DEV bool mbar_wait_short(uint64_t *bar, uint32_t parity, int *err, int code) {
+    if (mbar_test_wait(bar, parity)) return true;
+    for (int i = 0; i < 256; ++i)
+        if (mbar_try_wait(bar, parity)) return true;
+    return mbar_wait_bounded_ns(bar, parity, err, code, 1000000000ull);
+}
 CK_DEV bool mbar_wait_bounded(uint64_t *bar, uint32_t parity, int *err, int code) {
     return mbar_wait_bounded_ns(bar, parity, err, code, 1000000000ull);
 }

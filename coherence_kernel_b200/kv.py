@@ -21,18 +21,29 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .ops import TYPE_NUMBERS, _dev, _ptr, _stream
+from .ops import _FLOATS, TYPE_NUMBERS, _call, _dev, _ptr, _stream
 
 
 @dataclass
 class Plan:
-    """What ck_kv_plan wrote: one step's view of the cache."""
+    """What ck_kv_plan wrote: one step's view of the cache.  Its buffers are checked once, here."""
     length: torch.Tensor      # int32 [nreq] tokens held
     kv_len: torch.Tensor      # int32 [nreq] tokens the request's rows attend over (0: not served)
     q_start: torch.Tensor     # int32 [nreq + 1] first row of each request
     slots: torch.Tensor       # int64 [ntok] cache slot of every row, -1 for none
     positions: torch.Tensor   # int32 [ntok] position in its request, -1 for none
     free_count: torch.Tensor  # int32 [1] free pages left
+
+    def __post_init__(self):
+        n = self.length.numel()
+        for t, name, dt, k in ((self.length, "length", torch.int32, n), (self.kv_len, "kv_len", torch.int32, n),
+                               (self.q_start, "q_start", torch.int32, n + 1),
+                               (self.slots, "slots", torch.int64, self.slots.numel()),
+                               (self.positions, "positions", torch.int32, self.slots.numel()),
+                               (self.free_count, "free_count", torch.int32, 1)):
+            _dev(t, name, dt, k)
+            if t.device != self.length.device:
+                raise ValueError("the plan's buffers must be on one device")
 
 
 def plan_buffers(nreq: int, ntok: int, device) -> Plan:
@@ -41,87 +52,81 @@ def plan_buffers(nreq: int, ntok: int, device) -> Plan:
     return Plan(i(nreq), i(nreq), i(nreq + 1), torch.empty(ntok, dtype=torch.int64, device=device), i(ntok), i(1))
 
 
-def _same_device(*tensors):
-    dev = tensors[0].device
-    for t in tensors:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device}")
-    return torch.cuda.device(dev)
+_I32 = torch.int32
 
 
-def _rows(t, name, dtype, *inner):
-    """A tensor [n, *inner] whose rows are contiguous; returns its row stride in elements."""
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor")
-    if t.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
-        raise ValueError(f"{name} has dtype {t.dtype}, expected {dtype}")
-    if t.dim() != 1 + len(inner) or tuple(t.shape[1:]) != tuple(inner):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected [n, {', '.join(map(str, inner))}]")
-    step = 1
-    for size, stride in zip(reversed(inner), reversed(t.stride()[1:])):
-        if size != 1 and stride != step:
-            raise ValueError(f"{name}'s rows must be contiguous")
-        step *= size
-    if t.shape[0] > 1 and t.stride(0) < step:
-        raise ValueError(f"{name}'s rows overlap")
-    return t.stride(0) if t.shape[0] > 1 else step
+def _ints(t, name, n, device):
+    """A contiguous int32 tensor of at least n elements on the device; returns its address."""
+    if t.dtype is not _I32 or t.device != device or not t.is_contiguous() or t.numel() < n:
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} elements on {device}")
+    return t.data_ptr()
+
+
+def _rows3(t, name, shape, kinds, device):
+    """A tensor [n, heads, dim] of this shape with contiguous rows; returns the row stride."""
+    st = t.stride()
+    if t.shape != shape or t.dtype not in kinds or t.device != device:
+        raise ValueError(f"{name} must be {list(shape)} on {device}, of {' or '.join(map(str, kinds))}")
+    n, h, d = shape
+    if (st[2] != 1 and d > 1) or (st[1] != d and h > 1) or (n > 1 and st[0] < h * d):
+        raise ValueError(f"{name}'s rows must be contiguous")
+    return st[0] if n > 1 else h * d
+
+
+def _table(t, device):
+    st = t.stride()
+    n, w = t.shape
+    if t.dtype is not _I32 or t.device != device or (w > 1 and st[1] != 1) or (n > 1 and st[0] < w):
+        raise ValueError(f"table must be int32 [nreq, max_blocks] on {device} with contiguous rows")
+    return st[0] if n > 1 else w
 
 
 def plan(table, length, new_tokens, free_blocks, free_count, block_tokens: int, ntok: int, out: Plan | None = None) -> Plan:
     """Block tables and slot maps of one step (ck_kv_plan): table int32 [nreq, max_blocks] and
     free_blocks int32 [n_blocks] are updated in place; length and free_count are read, and the new
     ones are in the returned plan (whose tensors may be these)."""
+    dev = table.device
+    if not table.is_cuda or table.dim() != 2:
+        raise ValueError("table must be a CUDA tensor [nreq, max_blocks]")
     nreq, max_blocks = table.shape
-    stride = _rows(table, "table", torch.int32, max_blocks)
-    _dev(length, "length", torch.int32, nreq)
-    _dev(new_tokens, "new_tokens", torch.int32, nreq)
-    _dev(free_blocks, "free_blocks", torch.int32, 1)
-    _dev(free_count, "free_count", torch.int32, 1)
-    o = out if out is not None else plan_buffers(nreq, ntok, table.device)
-    for t, n, dt, k in ((o.length, "out.length", torch.int32, nreq), (o.kv_len, "out.kv_len", torch.int32, nreq),
-                        (o.q_start, "out.q_start", torch.int32, nreq + 1), (o.slots, "out.slots", torch.int64, ntok),
-                        (o.positions, "out.positions", torch.int32, ntok),
-                        (o.free_count, "out.free_count", torch.int32, 1)):
-        _dev(t, n, dt, k)
-    with _same_device(table, length, new_tokens, free_blocks, free_count, o.length, o.kv_len, o.q_start, o.slots,
-                      o.positions, o.free_count):
-        _lib.check(_lib.load().ck_kv_plan(_ptr(length), _ptr(new_tokens), nreq, _ptr(table), stride, max_blocks,
-                                          _ptr(free_blocks), _ptr(free_count), free_blocks.numel(), block_tokens, ntok,
-                                          _ptr(o.length), _ptr(o.free_count), _ptr(o.kv_len), _ptr(o.q_start),
-                                          _ptr(o.slots), _ptr(o.positions), _stream()), "ck_kv_plan")
+    stride = _table(table, dev)
+    o = out if out is not None else plan_buffers(nreq, ntok, dev)
+    if o.length.numel() < nreq or o.slots.numel() < ntok or o.length.device != dev:
+        raise ValueError(f"out holds less than {nreq} requests and {ntok} rows, or is not on {dev}")
+    _call("ck_kv_plan", dev, _ints(length, "length", nreq, dev), _ints(new_tokens, "new_tokens", nreq, dev), nreq,
+          table.data_ptr(), stride, max_blocks, _ints(free_blocks, "free_blocks", 1, dev),
+          _ints(free_count, "free_count", 1, dev), free_blocks.numel(), block_tokens, ntok, o.length.data_ptr(),
+          o.free_count.data_ptr(), o.kv_len.data_ptr(), o.q_start.data_ptr(), o.slots.data_ptr(),
+          o.positions.data_ptr())
     return o
 
 
 def _config(k_cache, v_cache):
     """ck_kv_config of cache tensors [n_blocks, block_tokens, n_kv_heads, head_dim] (any strides with
     contiguous heads, so a [n_blocks, n_kv_heads, block_tokens, head_dim] cache is passed permuted)."""
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
-        raise ValueError("k_cache and v_cache must be 4-dimensional, of one shape and type")
-    if k_cache.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"the cache has dtype {k_cache.dtype}, expected bfloat16 or float16")
-    if not k_cache.is_cuda or not v_cache.is_cuda:
-        raise ValueError("the cache must be CUDA tensors")
-    if k_cache.stride() != v_cache.stride() or k_cache.stride(3) != 1:
-        raise ValueError("k_cache and v_cache need the same strides and contiguous heads")
+    kt, st = k_cache.dtype, k_cache.stride()
+    if len(st) != 4 or k_cache.shape != v_cache.shape or kt != v_cache.dtype or st != v_cache.stride() or st[3] != 1:
+        raise ValueError("k_cache and v_cache must be 4-dimensional, of one shape, type and strides, heads contiguous")
+    if kt is not torch.bfloat16 and kt is not torch.float16:
+        raise ValueError(f"the cache has dtype {kt}, expected bfloat16 or float16")
+    if not k_cache.is_cuda or v_cache.device != k_cache.device:
+        raise ValueError("the cache must be CUDA tensors on one device")
     nb, bt, h, d = k_cache.shape
-    sb, st, sh, _ = k_cache.stride()
-    return _lib.KvConfig(h, d, bt, nb, TYPE_NUMBERS[k_cache.dtype], 0, sb, st, sh)
+    return _lib.KvConfig(h, d, bt, nb, TYPE_NUMBERS[kt], 0, st[0], st[1], st[2])
 
 
 def append(k, v, k_cache, v_cache, slots):
     """K/V rows [ntok, n_kv_heads, head_dim] (f32, f16 or bf16) into the cache at `slots` (int64 [ntok],
     distinct; those outside the cache are skipped), rounded to the cache's type (ck_kv_append)."""
     cfg = _config(k_cache, v_cache)
-    kinds = (torch.float32, torch.float16, torch.bfloat16)
-    ks = _rows(k, "k", kinds, cfg.n_kv_heads, cfg.head_dim)
-    vs = _rows(v, "v", k.dtype, cfg.n_kv_heads, cfg.head_dim)
-    ntok = k.shape[0]
-    if v.shape[0] != ntok:
-        raise ValueError("k and v have different numbers of rows")
-    _dev(slots, "slots", torch.int64, ntok)
-    with _same_device(k, v, k_cache, v_cache, slots):
-        _lib.check(_lib.load().ck_kv_append(ctypes.byref(cfg), TYPE_NUMBERS[k.dtype], _ptr(k), ks, _ptr(v), vs,
-                                            _ptr(slots), ntok, _ptr(k_cache), _ptr(v_cache), _stream()), "ck_kv_append")
+    dev, ntok = k_cache.device, k.shape[0]
+    shape = (ntok, cfg.n_kv_heads, cfg.head_dim)
+    ks = _rows3(k, "k", shape, _FLOATS, dev)
+    vs = _rows3(v, "v", shape, (k.dtype,), dev)
+    if slots.dtype is not torch.int64 or slots.device != dev or slots.numel() < ntok or not slots.is_contiguous():
+        raise ValueError(f"slots must be a contiguous int64 tensor of {ntok} elements on {dev}")
+    _call("ck_kv_append", dev, ctypes.byref(cfg), TYPE_NUMBERS[k.dtype], k.data_ptr(), ks, v.data_ptr(), vs,
+          slots.data_ptr(), ntok, k_cache.data_ptr(), v_cache.data_ptr())
 
 
 class PagedAttention:
@@ -143,31 +148,32 @@ class PagedAttention:
         """q [ntok, n_heads, head_dim] in the cache's type or f32 -> out of q's type (and lse fp32
         [ntok, n_heads] with return_lse).  Rows from q_start[nreq] on are not written."""
         cfg = _config(k_cache, v_cache)
-        if (cfg.n_kv_heads, cfg.head_dim) != (self.n_kv_heads, self.head_dim):
-            raise ValueError("the cache's heads are not those this object was made for")
-        qs = _rows(q, "q", (torch.float32, k_cache.dtype), self.n_heads, self.head_dim)
+        heads, dim, dev = self.n_heads, self.head_dim, k_cache.device
+        if cfg.n_kv_heads != self.n_kv_heads or cfg.head_dim != dim or self.ws.device != dev:
+            raise ValueError("the cache's heads or device are not those this object was made for")
         ntok = q.shape[0]
         nreq, max_blocks = table.shape
         if ntok > self.max_tokens or nreq > self.max_requests:
             raise ValueError("more rows or requests than this object was made for")
-        ts = _rows(table, "table", torch.int32, max_blocks)
-        _dev(kv_len, "kv_len", torch.int32, nreq)
-        _dev(q_start, "q_start", torch.int32, nreq + 1)
+        shape = (ntok, heads, dim)
+        qs = _rows3(q, "q", shape, (k_cache.dtype, torch.float32), dev)
         if out is None:
-            out = torch.empty((ntok, self.n_heads, self.head_dim), dtype=q.dtype, device=q.device)
-        os_ = _rows(out, "out", q.dtype, self.n_heads, self.head_dim)
-        if out.shape[0] < ntok:
-            raise ValueError("out has fewer rows than q")
-        if return_lse and lse is None:
-            lse = torch.empty((ntok, self.n_heads), dtype=torch.float32, device=q.device)
-        if lse is not None:
-            _dev(lse, "lse", torch.float32, ntok * self.n_heads)
-        with _same_device(q, k_cache, v_cache, table, kv_len, q_start, out, lse, self.ws):
-            _lib.check(_lib.load().ck_paged_attention(
-                ctypes.byref(cfg), self.n_heads, TYPE_NUMBERS[q.dtype], _ptr(q), qs, _ptr(k_cache), _ptr(v_cache),
-                _ptr(table), ts, max_blocks, _ptr(kv_len), _ptr(q_start), nreq, ntok,
-                1.0 / math.sqrt(self.head_dim) if scale is None else scale, int(causal), window, _ptr(out), os_,
-                _ptr(lse), _ptr(self.ws), self.ws_bytes, _stream()), "ck_paged_attention")
+            out = torch.empty(shape, dtype=q.dtype, device=dev)
+            os_ = heads * dim
+        else:
+            os_ = _rows3(out, "out", shape, (q.dtype,), dev)
+        if lse is None:
+            if return_lse:
+                lse = torch.empty((ntok, heads), dtype=torch.float32, device=dev)
+        elif lse.device != dev:
+            raise ValueError(f"lse must be on {dev}")
+        else:
+            _dev(lse, "lse", torch.float32, ntok * heads)
+        _call("ck_paged_attention", dev, ctypes.byref(cfg), heads, TYPE_NUMBERS[q.dtype], q.data_ptr(), qs,
+              k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), _table(table, dev), max_blocks,
+              _ints(kv_len, "kv_len", nreq, dev), _ints(q_start, "q_start", nreq + 1, dev), nreq, ntok,
+              1.0 / math.sqrt(dim) if scale is None else scale, int(causal), window, out.data_ptr(), os_,
+              None if lse is None else lse.data_ptr(), self.ws.data_ptr(), self.ws_bytes)
         return (out, lse) if return_lse else out
 
     def status(self):
@@ -198,10 +204,18 @@ class PagedKV:
         n = new_tokens.numel()
         if n > self.max_requests or ntok > self.max_tokens:
             raise ValueError("more requests or rows than the cache was made for")
-        o = out if out is not None else plan_buffers(n, ntok, self.k.device)
-        o.length, o.free_count = self.length[:n], self.free_count
+        if out is None:
+            b = plan_buffers(n, ntok, self.k.device)
+            out = Plan(self.length[:n], b.kv_len, b.q_start, b.slots, b.positions, self.free_count)
+        elif out.length.data_ptr() != self.length.data_ptr() or out.free_count.data_ptr() != self.free_count.data_ptr():
+            raise ValueError("out must come from this cache's step_buffers")
         return plan(self.table[:n], self.length[:n], new_tokens, self.free_blocks, self.free_count, self.block_tokens,
-                    ntok, out=o)
+                    ntok, out=out)
+
+    def step_buffers(self, nreq: int, ntok: int) -> Plan:
+        """Buffers for `plan` calls of nreq requests and ntok rows, over this cache's state (for captured steps)."""
+        b = plan_buffers(nreq, ntok, self.k.device)
+        return Plan(self.length[:nreq], b.kv_len, b.q_start, b.slots, b.positions, self.free_count)
 
     def append(self, k, v, plan: Plan):
         append(k, v, self.k, self.v, plan.slots)

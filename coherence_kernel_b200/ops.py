@@ -192,48 +192,79 @@ def route_dsv4(logits, bias, nused, wscale):
     return ids, wts
 
 
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _on(device):
+    """(device guard or None, the device's current stream): a guard only where the tensors lie on another
+    device than the current one, which a small call's time cannot hide."""
+    i = device.index
+    guard = None if i is None or i == torch.cuda.current_device() else torch.cuda.device(device)
+    return guard, torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if i is None else i)
+
+
+def _call(name, device, *args):
+    """The C call on the device's current stream, appended to the arguments; raises on an error code."""
+    guard, stream = _on(device)
+    fn = getattr(_lib.load(), name)
+    if guard is None:
+        rc = fn(*args, stream)
+    else:
+        with guard:
+            rc = fn(*args, stream)
+    if rc:
+        _lib.check(rc, name)
+
+
+def _matrix(t, name, device, shape):
+    """The row stride of a CUDA matrix of this shape with contiguous rows, on this device."""
+    if not t.is_cuda or t.device != device or t.dtype not in _FLOATS:
+        raise ValueError(f"{name} must be a CUDA tensor of f32, f16 or bf16 on {device}")
+    st = t.stride()
+    if t.shape != shape or (st[1] != 1 and shape[1] > 1) or (shape[0] > 1 and st[0] < shape[1]):
+        raise ValueError(f"{name} must be {tuple(shape)} with contiguous rows")
+    return st[0] if shape[0] > 1 else shape[1]
+
+
 def rmsnorm_add(x, residual, gain, eps, out_dtype=None, out=None, residual_out=None):
     """RMS norm with the residual's addition (ck_rmsnorm_add): s = x + residual (residual None: s = x),
     out = s / sqrt(mean(s^2) + eps) * gain.  x and residual are [ntok, hidden] (rows may be strided);
     s is stored to residual_out, by default the residual itself.  out_dtype: f32, f16, bf16 (default x's)
     or "q8_0", which returns the rows' GGUF blocks as uint8 [ntok, hidden // 32 * 34]."""
-    ntok, hidden = x.shape
-    kinds = (torch.float32, torch.float16, torch.bfloat16)
-    for t, n in ((x, "x"), (residual, "residual"), (residual_out, "residual_out")):
-        if t is None:
-            continue
-        if not t.is_cuda or t.dtype not in kinds:
-            raise ValueError(f"{n} must be a CUDA tensor of f32, f16 or bf16")
-        if tuple(t.shape) != (ntok, hidden) or (hidden > 1 and t.stride(1) != 1) or (ntok > 1 and t.stride(0) < hidden):
-            raise ValueError(f"{n} must be [{ntok}, {hidden}] with contiguous rows")
-        if t.device != x.device:
-            raise ValueError(f"{n} is on {t.device}, x on {x.device}")
-    _dev(gain, "gain", torch.float32, hidden)
-    if residual is None and residual_out is not None:
-        raise ValueError("residual_out without a residual")
+    shape, dev = x.shape, x.device
+    if len(shape) != 2:
+        raise ValueError("x must be [ntok, hidden]")
+    ntok, hidden = shape
+    xs = _matrix(x, "x", dev, shape)
+    rs, rt, rp, rop = 0, 0, None, None
     if residual is not None:
-        residual_out = residual if residual_out is None else residual_out
-        if residual_out.dtype != residual.dtype or (ntok > 1 and residual_out.stride(0) != residual.stride(0)):
-            raise ValueError("residual_out must have the residual's type and row stride")
-    out_dtype = (out.dtype if out is not None else x.dtype) if out_dtype is None else out_dtype
-    if out_dtype not in TYPE_NUMBERS:
+        rs, rt, rp = _matrix(residual, "residual", dev, shape), TYPE_NUMBERS[residual.dtype], residual.data_ptr()
+        rop = rp
+        if residual_out is not None:
+            if residual_out.dtype != residual.dtype or _matrix(residual_out, "residual_out", dev, shape) != rs:
+                raise ValueError("residual_out must have the residual's type and row stride")
+            rop = residual_out.data_ptr()
+    elif residual_out is not None:
+        raise ValueError("residual_out without a residual")
+    _dev(gain, "gain", torch.float32, hidden)
+    if out_dtype is None:
+        out_dtype = out.dtype if out is not None else x.dtype
+    ot = TYPE_NUMBERS.get(out_dtype)
+    if ot is None:
         raise ValueError(f"unsupported out_dtype {out_dtype}")
-    if out_dtype == "q8_0":
+    if ot == 8:
         if out is None:
-            out = torch.empty((ntok, hidden // 32 * Q8_0_BLOCK_BYTES), dtype=torch.uint8, device=x.device)
+            out = torch.empty((ntok, hidden // 32 * Q8_0_BLOCK_BYTES), dtype=torch.uint8, device=dev)
         _dev(out, "out", torch.uint8, ntok * (hidden // 32) * Q8_0_BLOCK_BYTES)
+        os_ = 0
     else:
         if out is None:
-            out = torch.empty((ntok, hidden), dtype=out_dtype, device=x.device)
-        if tuple(out.shape) != (ntok, hidden) or out.dtype != out_dtype or (hidden > 1 and out.stride(1) != 1) or \
-                (ntok > 1 and out.stride(0) < hidden):
-            raise ValueError(f"out must be {out_dtype} [{ntok}, {hidden}] with contiguous rows")
-    if gain.device != x.device or out.device != x.device:
+            out = torch.empty(shape, dtype=out_dtype, device=dev)
+        elif out.dtype != out_dtype:
+            raise ValueError(f"out has dtype {out.dtype}, expected {out_dtype}")
+        os_ = _matrix(out, "out", dev, shape)
+    if gain.device != dev or out.device != dev:
         raise ValueError("x, gain and out must be on one device")
-    row = lambda t: 0 if t is None else (t.stride(0) if ntok > 1 else hidden)
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.load().ck_rmsnorm_add(
-            TYPE_NUMBERS[x.dtype], _ptr(x), row(x), 0 if residual is None else TYPE_NUMBERS[residual.dtype],
-            _ptr(residual), _ptr(residual_out), row(residual), _ptr(gain), TYPE_NUMBERS[out_dtype], _ptr(out),
-            0 if out_dtype == "q8_0" else row(out), ntok, hidden, eps, _stream()), "ck_rmsnorm_add")
+    _call("ck_rmsnorm_add", dev, TYPE_NUMBERS[x.dtype], x.data_ptr(), xs, rt, rp, rop, rs, gain.data_ptr(), ot,
+          out.data_ptr(), os_, ntok, hidden, eps)
     return out

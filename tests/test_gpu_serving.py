@@ -471,7 +471,7 @@ def test_steps_together_and_captured():
         p = c.plan(i(prompt), 64)
         c.append(k_all[:64], v_all[:64], p)
         first = c.attend(q_all[:64], p)[:42].clone()
-        one, buf = i([1, 1, 1]), kv.plan_buffers(3, 3, "cuda")
+        one, buf = i([1, 1, 1]), c.step_buffers(3, 3)
         qs, ks, vs = q_all[:3].clone(), k_all[:3].clone(), v_all[:3].clone()
         out = torch.empty_like(qs)
 
