@@ -674,7 +674,8 @@ int ck_paged_attention(const ck_kv_config *c, uint32_t n_heads, int io_type, con
     const bool decode = ntok <= nreq && p.gd.d < ck::ATTN_CHUNK_ROWS;
     const bool chunk = !decode && ck::attn_chunk_ok_types(io_type, (int)c->cache_type, c->head_dim) &&
                        (uint64_t)ntok * p.gd.d >= ck::ATTN_CHUNK_ROWS;
-    p.row_split = chunk ? ck::ATTN_CHUNK_ROWS : ck::ATTN_NO_CHUNK;
+    // of a single request the chunk form takes what it gets, in one launch
+    p.row_split = !chunk ? ck::ATTN_NO_CHUNK : nreq == 1 ? 0 : ck::ATTN_CHUNK_ROWS;
     uint8_t *at = (uint8_t *)ws + 256;  // after the error word: each form's cuts, then its parts
     const auto take = [&](size_t bytes) { uint8_t *b = at; at += al(bytes); return b; };
     p.cuts = (ck::AttnCuts *)take(sizeof(ck::AttnCuts));
@@ -684,7 +685,7 @@ int ck_paged_attention(const ck_kv_config *c, uint32_t n_heads, int io_type, con
         g.cuts = (ck::AttnCuts *)take(sizeof(ck::AttnCuts));
         g.part_o = (float *)take(ck::attn_chunk_workspace_bytes(c->head_dim));
         rc = ck::launch_attn_chunk(g, S(s));
-        if (rc) return fail(rc, "ck_paged_attention");
+        if (rc || nreq == 1) return fail(rc, "ck_paged_attention");
     }
     return fail(ck::launch_attn_few(p, S(s)), "ck_paged_attention");
 }

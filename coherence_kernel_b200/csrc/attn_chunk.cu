@@ -111,10 +111,24 @@ CK_DEV float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
+// queries: a 3D map (dim, head, token), a box of 64 dims of a group's heads for 128 / group tokens: 128 rows in tile order
+CK_DEV void tma_load_q(uint32_t dst, const CUtensorMap *map, uint64_t *bar, int d, int head, int tok) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"((uint64_t)map), "r"(smem_u32(bar)), "r"(d), "r"(head), "r"(tok)
+        : "memory");
+}
+inline int make_q_map(CUtensorMap *m, const AttnParams &p, int tokens) {
+    const cuuint64_t dims[3] = {p.head_dim, (cuuint64_t)p.n_kv * p.gd.d, p.ntok};
+    const cuuint64_t strides[2] = {p.head_dim * 2ull, p.q_stride * 2};
+    const cuuint32_t box[3] = {64, p.gd.d, (cuuint32_t)tokens};
+    return encode_map(m, p.q, p.cache_type, 3, dims, strides, box);
+}
+
 template <int TYPE, int DP, bool TMA>
 __global__ void __launch_bounds__(NTHREADS, 1)
     k_attn_chunk(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap kmap,
-                 const __grid_constant__ CUtensorMap vmap, int box) {
+                 const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap qmap, int box, int qbox) {
     using F = Chunk<DP>;
     constexpr int PIECES = DP / 8;           // 16-byte pieces of a row
     constexpr int ROWS_PER = 32 / PIECES;    // rows one warp instruction copies
@@ -122,6 +136,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     extern __shared__ uint8_t smem_raw[];
     __shared__ typename S::Shared sh;
     __shared__ uint32_t tmem_slot;
+    __shared__ uint32_t item_info[8];  // by item modulo 8: its units in this CTA, and 1 << 31 if both halves hold rows
     __shared__ uint32_t poison[8];  // item number + 1 of an item whose V was cleaned, by item modulo 8
     uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     Bars *bar = reinterpret_cast<Bars *>(smem + F::BAR_OFF);
@@ -144,7 +159,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             mbar_init(&bar->empty[i], 1);
             mbar_init(&bar->raw[i], 1);
         }
-        mbar_init(&bar->q_full, TMA ? 96 : 128);
+        mbar_init(&bar->q_full, qbox ? 1 : (TMA ? 96 : 128) + 1);
         mbar_init(&bar->q_empty, 1);
         for (int t = 0; t < 2; ++t) {
             mbar_init(&bar->s_full[t], 1);
@@ -167,7 +182,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 
     if (wg == 2) {
         // -------------------------------------------------------------------------------- loader
-        reg_dec<80>();
+        reg_dec<72>();
         const int w = warp - 8;
         constexpr uint32_t HALF = F::TILE / F::HALVES;
         typename S::Items it;
@@ -225,6 +240,10 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             }
             if (bad) poison[item & 7] = item + 1;
         };
+        // what the products' warp needs of an item, before the arrival that lets it at the queries
+        const auto describe = [&](uint32_t item) {
+            item_info[item & 7] = (uint32_t)(it.c1 - it.c0) | (uint32_t)(halves(p, it.q, it.at.t) - 1) << 31;
+        };
         uint32_t e = 0, item = 0;  // ring entries and items so far
         bool ok = true;
         if constexpr (TMA) {
@@ -266,8 +285,23 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                                     tma_load_kv(tile + x * HALF, map, full, x * 64, it.at.h, at.y, at.x);
                             }
                             __syncwarp();
+                            if (qbox && kv == 0 && c == it.c0) {
+                                ok = room(&bar->q_empty, (item & 1) ^ 1);
+                                if (!ok) break;
+                                if (lane == 0) {
+                                    describe(item);
+                                    const int nh = halves(p, it.q, it.at.t), tok = it.q.q0 + (it.at.t * 2) * qbox;
+                                    mbar_arrive_expect_tx(&bar->q_full, nh * F::TILE);
+                                    for (int t = 0; t < nh; ++t)
+                                        for (int x = 0; x < F::HALVES; ++x)
+                                            tma_load_q(sbase + F::Q_OFF + t * F::TILE + x * HALF, &qmap, &bar->q_full,
+                                                       x * 64, it.at.h * p.gd.d, tok + t * qbox);
+                                }
+                                __syncwarp();
+                            }
                         }
                     }
+                    ++item;
                 } while (ok && it.next(p));
                 // after a wait gave up, no load outlives the block
                 for (uint32_t x = e > NS ? e - NS : 0; !ok && x < e; ++x) {
@@ -280,10 +314,16 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                 const int me = threadIdx.x - 288;  // 0 .. 95
                 uint32_t raw_parity = 0;           // a bit per stage
                 do {
-                    ok = room(&bar->q_empty, (item & 1) ^ 1);
-                    if (!ok) break;
-                    for (int b = w - 1; b < TR / 32; b += 3) copy_queries(b);
-                    hand_over(&bar->q_full);
+                    if (!qbox) {
+                        ok = room(&bar->q_empty, (item & 1) ^ 1);
+                        if (!ok) break;
+                        for (int b = w - 1; b < TR / 32; b += 3) copy_queries(b);
+                        hand_over(&bar->q_full);
+                        if (me == 0) {
+                            describe(item);
+                            mbar_arrive(&bar->q_full);
+                        }
+                    }
                     int all_lo, all_hi;
                     item_limits(p, it.q, it.at.t, all_lo, all_hi);
                     for (int c = it.c0; c < it.c1 && ok; ++c, e += 2) {
@@ -336,6 +376,10 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                             copy_queries(2 * w);
                             copy_queries(2 * w + 1);
                             hand_over(&bar->q_full);
+                            if (threadIdx.x == 256) {
+                                describe(item);
+                                mbar_arrive(&bar->q_full);
+                            }
                         }
                     }
                 }
@@ -346,15 +390,13 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         cp_wait<0>();  // no copy outlives the thread, also after a wait gave up
     } else if (wg == 3) {
         // ---------------------------------------------------------------------------- the products
-        reg_dec<64>();
+        reg_dec<72>();
         if (warp == 12) {
             constexpr uint32_t id_s = idesc16(TYPE, 128, KC, 0), id_o = idesc16(TYPE, 128, DP, 1);
             constexpr uint32_t HALF = F::TILE / F::HALVES;
             const uint64_t q_desc = sdesc_k_sw128(sbase + F::Q_OFF), k_desc = sdesc_k_sw128(sbase + F::RING_OFF),
                            v_desc = sdesc_n_sw128(sbase + F::RING_OFF, HALF);
             constexpr uint32_t STAGE16 = F::TILE >> 4;  // descriptors count 16 bytes
-            typename S::Items it;
-            it.set(p, pos, geo, n);
             const auto commit = [&](uint64_t *b) {
                 if (elect_one()) umma_commit(b);
                 __syncwarp();
@@ -404,10 +446,12 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             };
             uint32_t e = 0, item = 0, handed[2] = {0, 0};  // ring entries, items, P tiles taken from each half
             bool ok = true;
-            do {
-                const int nh = halves(p, it.q, it.at.t), units = it.c1 - it.c0;
+            for (int left = n; left > 0 && ok;) {
                 ok = wait_tile(&bar->q_full, item & 1, 31) && wait_tile(&bar->full[e % NS], (e / NS) & 1, 32);
                 if (!ok) break;
+                const uint32_t info = item_info[item & 7];
+                const int nh = 1 + (int)(info >> 31), units = (int)(info & 0x7fffffffu);
+                left -= units;
                 for (int t = 0; t < nh; ++t) scores(t, e % NS, t == nh - 1, t == nh - 1 && units == 1);
                 ++e;
                 for (int c = 0; c < units && ok; ++c) {
@@ -430,7 +474,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                     e += last ? 1 : 2;
                 }
                 ++item;
-            } while (ok && it.next(p));
+            }
             // every product has completed before tensor memory is freed, also after a wait gave up
             commit(&bar->done);
             mbar_wait_short(&bar->done, 0, nullptr, 0);
@@ -650,10 +694,14 @@ int launch(AttnParams p, int box, cudaStream_t s) {
     }
     const uint32_t grid = SMS;
     p.part_ml = p.part_o + (size_t)grid * 2 * TR * DP;
-    CUtensorMap kmap = {}, vmap = {};
+    CUtensorMap kmap = {}, vmap = {}, qmap = {};
+    // queries by TMA too where a 128-row tile is whole tokens of the group's heads (powers of two up to 128)
+    const uint32_t group = p.gd.d;
+    const int qbox = TMA && group <= 128 && (group & (group - 1)) == 0 ? 128 / (int)group : 0;
+    if (qbox && make_q_map(&qmap, p, qbox)) return CK_ERR_ARG;
     cudaError_t e;
     if (TMA && (make_kv_map(&kmap, p.k, p, box) || make_kv_map(&vmap, p.v, p, box))) return CK_ERR_ARG;
-    e = launch_pdl(k_attn_chunk<TYPE, DP, TMA>, dim3(grid), dim3(NTHREADS), F::SMEM, s, p, kmap, vmap, box);
+    e = launch_pdl(k_attn_chunk<TYPE, DP, TMA>, dim3(grid), dim3(NTHREADS), F::SMEM, s, p, kmap, vmap, qmap, box, qbox);
     if (e == cudaSuccess) e = launch_pdl(k_attn_join_chunk<DP>, dim3(grid - 1, DP / 8), dim3(TR), 0, s, p);
     return (int)e;
 }

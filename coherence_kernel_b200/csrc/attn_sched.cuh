@@ -264,7 +264,8 @@ inline int kv_box(uint32_t block_tokens, int most) {
     while (b >= 8 && block_tokens % b) b >>= 1;
     return b >= 8 ? b : 0;
 }
-inline int make_kv_map(CUtensorMap *m, const void *base, const AttnParams &p, int box) {
+inline int encode_map(CUtensorMap *m, const void *base, int type, cuuint32_t rank, const cuuint64_t *dims,
+                      const cuuint64_t *strides, const cuuint32_t *box) {
     using Fn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                             const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -277,14 +278,18 @@ inline int make_kv_map(CUtensorMap *m, const void *base, const AttnParams &p, in
                    : nullptr;
     }();
     if (!enc) return CK_ERR_NODEV;
-    const cuuint64_t dims[4] = {p.head_dim, p.n_kv, p.btd.d, p.n_blocks};
-    const cuuint64_t strides[3] = {p.head_stride * 2, p.token_stride * 2, p.block_stride * 2};
-    const cuuint32_t box4[4] = {64, 1, (cuuint32_t)box, 1}, one[4] = {1, 1, 1, 1};
-    const CUresult r = enc(m, p.cache_type == T_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-                           const_cast<void *>(base), dims, strides, box4, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    const cuuint32_t one[4] = {1, 1, 1, 1};
+    const CUresult r = enc(m, type == T_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
+                           const_cast<void *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? 0 : CK_ERR_ARG;
+}
+inline int make_kv_map(CUtensorMap *m, const void *base, const AttnParams &p, int box) {
+    const cuuint64_t dims[4] = {p.head_dim, p.n_kv, p.btd.d, p.n_blocks};
+    const cuuint64_t strides[3] = {p.head_stride * 2, p.token_stride * 2, p.block_stride * 2};
+    const cuuint32_t box4[4] = {64, 1, (cuuint32_t)box, 1};
+    return encode_map(m, base, p.cache_type, 4, dims, strides, box4);
 }
 
 // The keys that row's token may see: [lo, hi).
