@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         const int w = warp - 8;
         constexpr uint32_t HALF = F::TILE / F::HALVES;
         typename S::Items it;
-        it.set(p, pos, geo, n);
+        it.set(p, sh, n);
         const auto room = [&](uint64_t *b, uint32_t parity) -> bool {
             return __all_sync(0xffffffffu, mbar_wait_short(b, parity, p.err, 30));
         };
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 lanes: lane number << 16
         const uint32_t s_at = tmem + s_col(t) + lanes, o_at = tmem + o_col(t) + lanes;
         typename S::Items it;
-        it.set(p, pos, geo, n);
+        it.set(p, sh, n);
         uint32_t taken = 0, joined = 0;  // score tiles and outputs taken
         uint32_t item = 0;
         int segment = 0;

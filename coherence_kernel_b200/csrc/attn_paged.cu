@@ -37,8 +37,9 @@ struct Few {
     static constexpr int STAGES = DP <= 64 ? 4 : 3;
     static constexpr int STAGE = 2 * WK * ROW;
     static constexpr int RING = WARPS * STAGES * STAGE;
-    // the query tile (all terms), and after the last key the 16 x DP fp32 sum over the warps
-    static constexpr int QO = (TERMS * ROW > DP * 4 ? TERMS * ROW : DP * 4) * TR;
+    // the query tile (all terms), and after the last key two 16 x DP fp32 sums over two warps each
+    static constexpr int QO = DP * 8 * TR;
+    static_assert(TERMS * ROW <= DP * 8, "the query tile's terms");
     static constexpr int SMEM = RING + QO;
     static constexpr int CTAS = DP <= 64 ? 3 : DP <= 128 ? 2 : 1;  // per SM
 };
@@ -119,7 +120,7 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
     if (!part) return;
     const int n = (int)(S::start(U, C, blockIdx.x + 1) - S::start(U, C, blockIdx.x));
     typename S::Items use, fill;
-    use.set(p, pos, geo, n);
+    use.set(p, sh, n);
     fill = use;
     int fill_c = fill.c0;
 
@@ -242,9 +243,11 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
             const int j0 = use.g.lo + c * KC + warp * WK;
             if (j0 >= use.g.hi) continue;
             const uint32_t kb = ring + (i % NS) * F::STAGE, vb = kb + WK * ROW;
-            float s[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-#pragma unroll
+            // even and odd steps into sums of their own: half the chain of dependent products
+            float s[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, s1[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll 2
             for (int ks = 0; ks < DP / 16; ++ks) {
+                float(&sk)[2][4] = (ks & 1) ? s1 : s;
                 uint32_t b[4];
                 {  // keys 0-7 | 8-15 by the 16 dims of this step
                     const int key = (lane & 7) + ((lane >> 4) << 3), c = ks * 2 + ((lane >> 3) & 1);
@@ -255,10 +258,14 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
                     uint32_t a[4];
                     const int r = lane & 15, c = ks * 2 + (lane >> 4);
                     ldsm4(qs + term * TR * ROW + r * ROW + ((c ^ (r & 7)) << 4), a);
-                    mma<TYPE>(s[0], a, b[0], b[1]);
-                    mma<TYPE>(s[1], a, b[2], b[3]);
+                    mma<TYPE>(sk[0], a, b[0], b[1]);
+                    mma<TYPE>(sk[1], a, b[2], b[3]);
                 }
             }
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[t][e] += s1[t][e];
             const bool partial = j0 < all_lo || j0 + WK > all_hi;  // some row does not see some key
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -342,15 +349,18 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
                 for (int w = 1; w < WARPS; ++w) mm = fmaxf(mm, wm[w][r]);
                 f[k] = ex2(m[k] - (mm == -INFINITY ? 0.0f : mm));
             }
-            for (int w = 0; w < WARPS; ++w) {
-                if (warp == w) {
+            // warps 0 and 1 lay their sums down, 2 and 3 add theirs to them
+#pragma unroll
+            for (int pass = 0; pass < 2; ++pass) {
+                if ((warp >> 1) == pass) {
 #pragma unroll
                     for (int d = 0; d < DP / 8; ++d)
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
-                            float2 *at = reinterpret_cast<float2 *>(osum + ((lane >> 2) + 8 * k) * DP + d * 8 + (lane & 3) * 2);
+                            float2 *at = reinterpret_cast<float2 *>(osum + ((warp & 1) * TR + (lane >> 2) + 8 * k) * DP +
+                                                                    d * 8 + (lane & 3) * 2);
                             float2 v = make_float2(o[d][2 * k] * f[k], o[d][2 * k + 1] * f[k]);
-                            if (w) v.x += at->x, v.y += at->y;
+                            if (pass) v.x += at->x, v.y += at->y;
                             *at = v;
                         }
                 }
@@ -376,7 +386,7 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
                     float v[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        v[e] = osum[r * DP + c * 8 + e] * inv;
+                        v[e] = (osum[r * DP + c * 8 + e] + osum[(TR + r) * DP + c * 8 + e]) * inv;
                         if (any_bad)  // TERMS > 1: every step's V was cleaned
                             v[e] += nonfinite_v(p, use.at.r, use.at.h, c * 8 + e, use.g.lo + use.c0 * KC,
                                                 min(use.g.lo + use.c1 * KC, use.g.hi), WK, TERMS > 1 ? 0x7fffffff : all_lo,

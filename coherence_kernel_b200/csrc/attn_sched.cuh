@@ -66,7 +66,11 @@ struct Sched {
     }
     // units of request r (all 32 lanes of a warp call this together, each with its own request)
     static CK_DEV long long units(const AttnParams &p, int r) {
-        Req q = {0, 0, 0};
+        Req q;
+        return units(p, r, q);
+    }
+    static CK_DEV long long units(const AttnParams &p, int r, Req &q) {
+        q = {0, 0, 0};
         if (r < (int)p.nreq) q = load_req(p, r);
         const int nt = r < (int)p.nreq ? tiles(p, q) : 0;
         long long n = 0;
@@ -90,6 +94,7 @@ struct Sched {
         long long before;
         Pos pos;
         Geo geo;
+        Req req;
     };
     // exclusive prefix of v over the CTA; `all` receives the sum
     static CK_DEV long long scan(long long v, Shared &sh, long long &all) {
@@ -110,66 +115,75 @@ struct Sched {
         __syncthreads();
         return before + s - v;
     }
-    static CK_DEV long long start(long long U, int C, int c) { return U * c / C; }
+    // U c / C; a 64-bit division is a hundred instructions, and few batches need it (C < 512)
+    static CK_DEV long long start(long long U, int C, int c) {
+        return U < 1 << 22 ? (long long)((uint32_t)U * (uint32_t)c / (uint32_t)C) : U * c / C;
+    }
 
     // Called by the whole CTA.  Finds the total U, the CTAs that take part C = min(grid, U), and the
     // position of unit start(cta); returns false when cta takes no part.
     static CK_DEV bool find(const AttnParams &p, Shared &sh, int grid, int cta, long long &U, int &C, Pos &pos, Geo &geo) {
         const int n = (int)p.nreq, bd = (int)blockDim.x;
-        long long mine = units(p, threadIdx.x), all = 0, sum = mine;
+        Req q;
+        long long mine = units(p, threadIdx.x, q), sum = mine;
         for (int b = bd; b < n; b += bd) sum += units(p, b + (int)threadIdx.x);
-        scan(sum, sh, U);
+        long long ex = scan(sum, sh, U);
         C = (int)(U < grid ? U : grid);
         if (cta >= C) return false;
         const long long u = start(U, C, cta);
-        long long base = 0;
-        for (int b = 0;; b += bd) {
-            if (b) mine = units(p, b + (int)threadIdx.x);
-            const long long ex = base + scan(mine, sh, all);
-            if (u < base + all) {
-                if (u >= ex && u < ex + mine) {
-                    sh.pos.r = b + (int)threadIdx.x;
-                    sh.before = u - ex;
-                }
-                break;
+        if (n > bd) {  // more requests than threads: once more, block by block
+            long long base = 0, all = 0;
+            for (int b = 0;; b += bd) {
+                mine = units(p, b + (int)threadIdx.x, q);
+                ex = base + scan(mine, sh, all);
+                if (u >= ex && u < ex + mine) sh.pos.r = b + (int)threadIdx.x;
+                if (u < base + all) break;
+                base += all;
             }
-            base += all;
+        } else if (u >= ex && u < ex + mine) {
+            sh.pos.r = (int)threadIdx.x;
+        }
+        if (u >= ex && u < ex + mine) {  // one thread: its request holds the unit
+            sh.before = u - ex;
+            sh.req = q;
+            if (tiles(p, q) == 1) place(p, sh, q, 0, tile_geo<TR, KC, ALIGN>(p, q, 0), (int)(u - ex));
         }
         __syncthreads();
-        if (threadIdx.x < 32) {  // the tile of the request: 32 at a time
-            const int lane = threadIdx.x;
-            const int r = sh.pos.r;
-            long long v = sh.before;
-            const Req q = load_req(p, r);
-            const int nt = tiles(p, q);
-            for (int tb = 0; tb < nt; tb += 32) {
-                const int t = tb + lane;
-                Geo g = {0, 0, 0};
-                if (t < nt) g = tile_geo<TR, KC, ALIGN>(p, q, t);
-                const long long m = (long long)g.nch * p.n_kv;
-                long long s = m;
-                for (int o = 1; o < 32; o <<= 1) {
-                    const long long x = __shfl_up_sync(0xffffffffu, s, o);
-                    if (lane >= o) s += x;
-                }
-                const long long tot = __shfl_sync(0xffffffffu, s, 31);
-                if (v < tot) {
-                    if (v >= s - m && v < s) {
-                        const int in = (int)(v - (s - m));
-                        sh.pos.t = t;
-                        sh.pos.h = in / g.nch;
-                        sh.pos.c = in - sh.pos.h * g.nch;
-                        sh.geo = g;
+        const int nt = tiles(p, sh.req);
+        if (nt > 1) {
+            if (threadIdx.x < 32) {  // the tile of the request: 32 at a time
+                const int lane = threadIdx.x;
+                long long v = sh.before;
+                q = sh.req;
+                for (int tb = 0; tb < nt; tb += 32) {
+                    const int t = tb + lane;
+                    Geo g = {0, 0, 0};
+                    if (t < nt) g = tile_geo<TR, KC, ALIGN>(p, q, t);
+                    const long long m = (long long)g.nch * p.n_kv;
+                    long long s = m;
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const long long x = __shfl_up_sync(0xffffffffu, s, o);
+                        if (lane >= o) s += x;
                     }
-                    break;
+                    const long long tot = __shfl_sync(0xffffffffu, s, 31);
+                    if (v < tot) {
+                        if (v >= s - m && v < s) place(p, sh, q, t, g, (int)(v - (s - m)));
+                        break;
+                    }
+                    v -= tot;
                 }
-                v -= tot;
             }
+            __syncthreads();
         }
-        __syncthreads();
         pos = sh.pos;
         geo = sh.geo;
         return true;
+    }
+    static CK_DEV void place(const AttnParams &p, Shared &sh, const Req &q, int t, const Geo &g, int in) {
+        sh.pos.t = t;
+        sh.pos.h = in / g.nch;
+        sh.pos.c = in - sh.pos.h * g.nch;
+        sh.geo = g;
     }
 
     // A walk over a CTA's consecutive units, item by item: units c0 .. c1 - 1 of the item are the CTA's.
@@ -178,10 +192,10 @@ struct Sched {
         Req q;
         Geo g;
         int nt, left, c0, c1;
-        CK_DEV void set(const AttnParams &p, const Pos &pos, const Geo &geo, int n) {
-            at = pos;
-            g = geo;
-            q = load_req(p, pos.r);
+        CK_DEV void set(const AttnParams &p, const Shared &sh, int n) {
+            at = sh.pos;
+            g = sh.geo;
+            q = sh.req;
             nt = tiles(p, q);
             left = n;
             span();
