@@ -136,7 +136,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     extern __shared__ uint8_t smem_raw[];
     __shared__ typename S::Shared sh;
     __shared__ uint32_t tmem_slot;
-    __shared__ uint32_t item_info[8];  // by item modulo 8: its units in this CTA, and 1 << 31 if both halves hold rows
+    __shared__ uint32_t item_info[8];  // by item modulo 8: its units in this CTA, 1 << 30 if it is the last, 1 << 31 if both
+                                       // halves hold rows
     __shared__ uint32_t poison[8];  // item number + 1 of an item whose V was cleaned, by item modulo 8
     uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     Bars *bar = reinterpret_cast<Bars *>(smem + F::BAR_OFF);
@@ -153,6 +154,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     S::leave_cut(p, U, C, pos, geo);
     if (!part) return;
     const int n = (int)(S::start(U, C, blockIdx.x + 1) - S::start(U, C, blockIdx.x));
+    if (pos.c >= geo.nch && n <= geo.nch + S::EXTRA - pos.c) return;  // no unit with keys
     if (threadIdx.x == 0) {
         for (int i = 0; i < NS; ++i) {
             mbar_init(&bar->full[i], TMA ? 1 : 128);
@@ -242,7 +244,10 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         };
         // what the products' warp needs of an item, before the arrival that lets it at the queries
         const auto describe = [&](uint32_t item) {
-            item_info[item & 7] = (uint32_t)(it.c1 - it.c0) | (uint32_t)(halves(p, it.q, it.at.t) - 1) << 31;
+            // the last item: what is left ends with it
+            const bool last = it.left <= it.g.nch + S::EXTRA - it.c0;
+            item_info[item & 7] = (uint32_t)(it.c1 - it.c0) | (uint32_t)last << 30 |
+                                  (uint32_t)(halves(p, it.q, it.at.t) - 1) << 31;
         };
         uint32_t e = 0, item = 0;  // ring entries and items so far
         bool ok = true;
@@ -446,12 +451,12 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             };
             uint32_t e = 0, item = 0, handed[2] = {0, 0};  // ring entries, items, P tiles taken from each half
             bool ok = true;
-            for (int left = n; left > 0 && ok;) {
+            for (bool more = true; more && ok;) {
                 ok = wait_tile(&bar->q_full, item & 1, 31) && wait_tile(&bar->full[e % NS], (e / NS) & 1, 32);
                 if (!ok) break;
                 const uint32_t info = item_info[item & 7];
-                const int nh = 1 + (int)(info >> 31), units = (int)(info & 0x7fffffffu);
-                left -= units;
+                const int nh = 1 + (int)(info >> 31), units = (int)(info & 0x3fffffffu);
+                more = !(info >> 30 & 1);
                 for (int t = 0; t < nh; ++t) scores(t, e % NS, t == nh - 1, t == nh - 1 && units == 1);
                 ++e;
                 for (int c = 0; c < units && ok; ++c) {
@@ -656,7 +661,7 @@ __global__ void __launch_bounds__(TR) k_attn_join_chunk(const __grid_constant__ 
     grid_dep_wait();
     Joint jt;
     const int d = (int)blockIdx.y * 8;
-    if (d >= (int)p.head_dim || !find_joint(p, (int)blockIdx.x + 1, jt)) return;
+    if (d >= (int)p.head_dim || !find_joint<S>(p, (int)blockIdx.x + 1, jt)) return;
     const Req q = load_req(p, jt.at.r);
     const int r = threadIdx.x, row = jt.at.t * TR + r;
     if (row >= q.nq * (int)p.gd.d) return;

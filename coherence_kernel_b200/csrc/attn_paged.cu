@@ -120,9 +120,10 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
     if (!part) return;
     const int n = (int)(S::start(U, C, blockIdx.x + 1) - S::start(U, C, blockIdx.x));
     typename S::Items use, fill;
-    use.set(p, sh, n);
+    if (!use.set(p, sh, n)) return;
     fill = use;
     int fill_c = fill.c0;
+    bool to_fill = true;
 
     // lane l < 16 looks up key l of the warp's next 16: its element offset, or -1 to fill with zeros
     // (past the tile's last key, so that what the page holds there never meets a product)
@@ -148,15 +149,14 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
     int filled = 0;
     int64_t off = lookup();
     const auto fill_next = [&]() {
-        if (filled < n) {
+        if (to_fill) {
             copy_in(filled % NS, off);
-            if (++filled < n) {
-                if (++fill_c == fill.c1) {
-                    fill.next(p);
-                    fill_c = 0;
-                }
-                off = lookup();
+            ++filled;
+            if (++fill_c == fill.c1) {
+                to_fill = fill.next(p);
+                fill_c = 0;
             }
+            if (to_fill) off = lookup();
         }
         cp_commit();  // an empty group past the end keeps the count of groups in step
     };
@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(128) k_attn_join_few(const __grid_constant__ A
     grid_dep_trigger_small();
     grid_dep_wait();
     Joint jt;
-    if (!find_joint(p, (int)blockIdx.x + 1, jt)) return;
+    if (!find_joint<S>(p, (int)blockIdx.x + 1, jt)) return;
     const Req q = load_req(p, jt.at.r);
     const int r = (int)blockIdx.y, row = jt.at.t * TR + r;
     if (row >= q.nq * (int)p.gd.d) return;

@@ -1,7 +1,9 @@
 // attn_sched.cuh -- how the attention kernels share their work out over a fixed number of CTAs.
 //
 // An item is one tile of TR rows (rows = tokens x the query heads of one K/V head, token-major) of
-// one request and K/V head; a unit is KC consecutive keys of an item.  Units are numbered request
+// one request and K/V head; a unit is KC consecutive keys of an item.  An item also counts for EXTRA units without
+// keys at its end: what its queries' load and its epilogue cost, so that a CTA of many short items gets no more
+// work than one of a long one (64 ragged decodes, 1 to 8192 tokens: the slowest CTA took twice the median's time).  Units are numbered request
 // by request, tile by tile, head by head, key chunk by key chunk, and CTA c of C takes units
 // [c U / C, (c + 1) U / C): the split depends on the lengths alone, so ragged batches, one long
 // request and many short ones all fill the GPU evenly and results do not depend on timing.  An
@@ -59,6 +61,7 @@ struct Pos {
 template <int TR, int KC, bool CHUNK>
 struct Sched {
     static constexpr int ALIGN = CHUNK ? 64 : 16;
+    static constexpr int EXTRA = CHUNK ? 3 : 2;
     static CK_DEV int tiles(const AttnParams &p, const Req &q) {
         const int rows = q.nq * (int)p.gd.d;
         if (CHUNK ? rows < (int)p.row_split : rows >= (int)p.row_split) return 0;
@@ -75,14 +78,14 @@ struct Sched {
         const int nt = r < (int)p.nreq ? tiles(p, q) : 0;
         long long n = 0;
         if (nt <= 4)
-            for (int t = 0; t < nt; ++t) n += tile_geo<TR, KC, ALIGN>(p, q, t).nch;
+            for (int t = 0; t < nt; ++t) n += tile_geo<TR, KC, ALIGN>(p, q, t).nch + EXTRA;
         // requests of many tiles: the warp's lanes share them out
         for (uint32_t todo = __ballot_sync(0xffffffffu, nt > 4); todo; todo &= todo - 1) {
             const int src = __ffs(todo) - 1;
             const Req w = {0, __shfl_sync(0xffffffffu, q.nq, src), __shfl_sync(0xffffffffu, q.kl, src)};
             const int wt = __shfl_sync(0xffffffffu, nt, src);
             int part = 0;
-            for (int t = threadIdx.x & 31; t < wt; t += 32) part += tile_geo<TR, KC, ALIGN>(p, w, t).nch;
+            for (int t = threadIdx.x & 31; t < wt; t += 32) part += tile_geo<TR, KC, ALIGN>(p, w, t).nch + EXTRA;
             part = __reduce_add_sync(0xffffffffu, part);
             if ((int)(threadIdx.x & 31) == src) n = part;
         }
@@ -159,7 +162,7 @@ struct Sched {
                     const int t = tb + lane;
                     Geo g = {0, 0, 0};
                     if (t < nt) g = tile_geo<TR, KC, ALIGN>(p, q, t);
-                    const long long m = (long long)g.nch * p.n_kv;
+                    const long long m = t < nt ? (long long)(g.nch + EXTRA) * p.n_kv : 0;
                     long long s = m;
                     for (int o = 1; o < 32; o <<= 1) {
                         const long long x = __shfl_up_sync(0xffffffffu, s, o);
@@ -181,35 +184,33 @@ struct Sched {
     }
     static CK_DEV void place(const AttnParams &p, Shared &sh, const Req &q, int t, const Geo &g, int in) {
         sh.pos.t = t;
-        sh.pos.h = in / g.nch;
-        sh.pos.c = in - sh.pos.h * g.nch;
+        sh.pos.h = in / (g.nch + EXTRA);
+        sh.pos.c = in - sh.pos.h * (g.nch + EXTRA);
         sh.geo = g;
     }
 
-    // A walk over a CTA's consecutive units, item by item: units c0 .. c1 - 1 of the item are the CTA's.
+    // A walk over a CTA's consecutive units, item by item: units c0 .. c1 - 1 (with keys) of the item are the CTA's.
     struct Items {
         Pos at;
         Req q;
         Geo g;
         int nt, left, c0, c1;
-        CK_DEV void set(const AttnParams &p, const Shared &sh, int n) {
+        // false if the CTA has no unit with keys
+        CK_DEV bool set(const AttnParams &p, const Shared &sh, int n) {
             at = sh.pos;
             g = sh.geo;
             q = sh.req;
             nt = tiles(p, q);
             left = n;
-            span();
-        }
-        CK_DEV void span() {
             c0 = at.c;
             c1 = min(g.nch, c0 + left);
+            return c0 < g.nch || next(p);
         }
         CK_DEV bool whole() const { return c0 == 0 && c1 == g.nch; }
         // the next item; false at the end of the CTA's range
         CK_DEV bool next(const AttnParams &p) {
-            left -= c1 - c0;
+            left -= g.nch + EXTRA - c0;
             if (left <= 0) return false;
-            at.c = 0;
             if (++at.h >= (int)p.n_kv) {
                 at.h = 0;
                 if (++at.t >= nt) {
@@ -222,7 +223,8 @@ struct Sched {
                 }
                 g = tile_geo<TR, KC, ALIGN>(p, q, at.t);
             }
-            span();
+            c0 = 0;
+            c1 = min(g.nch, left);
             return true;
         }
     };
@@ -241,13 +243,14 @@ struct Sched {
 };
 
 // An item that spans CTAs, seen from boundary j (the start of CTA j's units): found at its first cut only.
-// Its parts are those of CTAs first .. first + n - 1, in each CTA's slot 0 except, where the item does not open
-// the first CTA's range, slot 1 there.
+// Its parts are those of CTAs first .. first + n - 1, in each CTA's slot 0 except, where the item is not the first
+// with keys in the first CTA's range, slot 1 there.
 struct Joint {
     Pos at;
     int first, n, slot0;
     CK_DEV size_t slot(int i) const { return (size_t)(first + i) * 2 + (i == 0 ? slot0 : 0); }
 };
+template <class S>
 CK_DEV bool find_joint(const AttnParams &p, int j, Joint &o) {
     const long long U = p.cuts->units;
     const int C = p.cuts->ctas;
@@ -255,10 +258,11 @@ CK_DEV bool find_joint(const AttnParams &p, int j, Joint &o) {
     const int4 v = p.cuts->at[j];
     const long long u = U * j / C, a = u - v.w, b = a + p.cuts->chunks[j];
     const long long before = U * (j - 1) / C;
-    if (v.w == 0 || before > a) return false;  // the cut is an item's start, or not its first
+    // the cut is an item's start, or behind its last keys, or not its first
+    if (v.w == 0 || v.w >= p.cuts->chunks[j] || before > a) return false;
     o.at = {v.x, v.y, v.z, v.w};
     o.first = j - 1;
-    o.slot0 = before == a ? 0 : 1;
+    o.slot0 = before >= a - S::EXTRA ? 0 : 1;  // a start behind the last item's keys is as good as a
     // the CTA of unit b - 1: the largest c with U c / C <= b - 1, that is c <= (C b - 1) / U
     o.n = (int)(((long long)C * b - 1) / U) - o.first + 1;
     return true;
