@@ -38,6 +38,14 @@ class KvConfig(ctypes.Structure):
                 ("head_stride", _u64)]
 
 
+class StepKv(ctypes.Structure):
+    """ck_step_kv (include/ck_b200.h)."""
+    _fields_ = [("cache", ctypes.POINTER(KvConfig)), ("k_cache", _p), ("v_cache", _p), ("table", _p),
+                ("table_stride", _u64), ("kv_len", _p), ("q_start", _p), ("slots", _p), ("max_blocks", _u32),
+                ("nreq", _u32), ("n_heads", _u32), ("window", _u32), ("scale", _f), ("workspace", _p),
+                ("workspace_bytes", _sz)]
+
+
 # name -> (restype, argtypes); every symbol include/*.h declares
 SIGNATURES = {
     "ck_last_error": (ctypes.c_char_p, []),
@@ -108,6 +116,8 @@ SIGNATURES = {
     "ck_decode_step_create": (_p, [ctypes.POINTER(DecodeConfig)] + [_p] * 15 + [_sz]),
     "ck_decode_step_run": (_i32, [_p, _p, _p, _p, _p, _u32, _p]),
     "ck_decode_step_capture": (_i32, [_p, _p, _p, _p, _p, _u32, _p]),
+    "ck_decode_step_run_kv": (_i32, [_p, _p, _p, _p, _p, _u32, ctypes.POINTER(StepKv), _p]),
+    "ck_decode_step_capture_kv": (_i32, [_p, _p, _p, _p, _p, _u32, ctypes.POINTER(StepKv), _p]),
     "ck_decode_step_replay": (_i32, [_p, _p]),
     "ck_decode_step_status": (_i32, [_p, _u32, _p]),
     "ck_decode_step_destroy": (None, [_p]),

@@ -13,6 +13,10 @@
 //   b  = bf16(rmsnorm(h, g_ffn))
 //   h += moe(b)                                ck_moe_layer_bf16 (route, permute, experts, combine)
 //
+// The form over a paged KV cache (ck_decode_step_run_kv) replaces the single position by attention over the
+// cached tokens: k and v are appended at the plan's slots, q attends over its request's pages, and the
+// residual's addition is part of the second norm.
+//
 // h is fp32 [ntok, hidden] and is updated in place; q, k, v are fp32 [ntok, hidden] outputs (the
 // rows a KV cache stores).  Every buffer the step needs beyond its inputs and outputs is carved
 // from one caller workspace.
@@ -103,6 +107,32 @@ struct ck_decode_step {
     cudaGraphExec_t exec;
 };
 
+namespace {
+// Records what `run` issues on the stream into the step's graph.
+template <typename Run>
+int capture(ck_decode_step *s, void *stream, Run run) {
+    if (!stream) return CK_EARG;  // the legacy default stream cannot be captured
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if (s->exec) {
+        cudaGraphExecDestroy(s->exec);
+        s->exec = nullptr;
+    }
+    cudaError_t e = cudaStreamBeginCapture(st, cudaStreamCaptureModeThreadLocal);
+    if (e != cudaSuccess) return (int)e;
+    const int rc = run();
+    cudaGraph_t g = nullptr;
+    e = cudaStreamEndCapture(st, &g);
+    if (rc) {
+        if (g) cudaGraphDestroy(g);
+        return rc;
+    }
+    if (e != cudaSuccess) return (int)e;
+    e = cudaGraphInstantiate(&s->exec, g, 0);
+    cudaGraphDestroy(g);
+    return (int)e;
+}
+}  // namespace
+
 extern "C" {
 
 size_t ck_decode_step_workspace_bytes(const ck_decode_config *c) {
@@ -174,25 +204,66 @@ int ck_decode_step_run(ck_decode_step *s, float *h_dev, float *q_dev, float *k_d
 
 int ck_decode_step_capture(ck_decode_step *s, float *h_dev, float *q_dev, float *k_dev, float *v_dev, uint32_t ntok,
                            void *stream) {
-    if (!s || !stream) return CK_EARG;  // the legacy default stream cannot be captured
+    if (!s) return CK_EARG;
+    return capture(s, stream, [&] { return ck_decode_step_run(s, h_dev, q_dev, k_dev, v_dev, ntok, stream); });
+}
+
+static int check_step_kv(const ck_decode_step *s, const ck_step_kv *kv) {
+    if (!kv || !kv->cache || !kv->k_cache_dev || !kv->v_cache_dev || !kv->table_dev || !kv->kv_len_dev ||
+        !kv->q_start_dev || !kv->slots_dev || !kv->workspace_dev)
+        return CK_EARG;
+    const ck_kv_config *c = kv->cache;
+    if (c->n_kv_heads == 0 || kv->n_heads % c->n_kv_heads || (uint64_t)kv->n_heads * c->head_dim != s->cfg.hidden)
+        return CK_ESHAPE;
+    return 0;
+}
+
+int ck_decode_step_run_kv(ck_decode_step *s, float *h_dev, float *q_dev, float *k_dev, float *v_dev, uint32_t ntok,
+                          const ck_step_kv *kv, void *stream) {
+    if (!s || !h_dev || !q_dev || !k_dev || !v_dev) return CK_EARG;
+    int rc = check_step_kv(s, kv);
+    if (rc) return rc;
+    if (ntok == 0) return 0;
+    if (ntok > s->cfg.max_tokens) return CK_ESHAPE;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (s->exec) {
-        cudaGraphExecDestroy(s->exec);
-        s->exec = nullptr;
+    const uint32_t H = s->cfg.hidden, KV = kv->cache->n_kv_heads * kv->cache->head_dim;
+    rc = ck_rmsnorm_add(CK_F32, h_dev, H, CK_F32, nullptr, nullptr, 0, s->g_attn, CK_F32, s->w.a, H, ntok, H, s->cfg.eps,
+                        stream);
+    // matrices of one shape share a launch where the tensor-core matvec applies
+    const uint8_t *wqkv[3] = {(const uint8_t *)s->wq, (const uint8_t *)s->wk, (const uint8_t *)s->wv};
+    float *yqkv[3] = {q_dev, k_dev, v_dev};
+    if (KV == H) {
+        if (!rc) rc = ck::launch_q4k_matvec_group(3, wqkv, s->w.a, yqkv, H, H, ntok, st);
+    } else {
+        if (!rc) rc = ck::launch_q4k_matvec(wqkv[0], s->w.a, q_dev, H, H, ntok, st);
+        if (!rc) rc = ck::launch_q4k_matvec_group(2, wqkv + 1, s->w.a, yqkv + 1, KV, H, ntok, st);
     }
-    cudaError_t e = cudaStreamBeginCapture(st, cudaStreamCaptureModeThreadLocal);
-    if (e != cudaSuccess) return (int)e;
-    const int rc = ck_decode_step_run(s, h_dev, q_dev, k_dev, v_dev, ntok, stream);
-    cudaGraph_t g = nullptr;
-    e = cudaStreamEndCapture(st, &g);
-    if (rc) {
-        if (g) cudaGraphDestroy(g);
-        return rc;
-    }
-    if (e != cudaSuccess) return (int)e;
-    e = cudaGraphInstantiate(&s->exec, g, 0);
-    cudaGraphDestroy(g);
-    return (int)e;
+    if (!rc)
+        rc = ck_kv_append(kv->cache, CK_F32, k_dev, KV, v_dev, KV, kv->slots_dev, ntok, kv->k_cache_dev, kv->v_cache_dev,
+                          stream);
+    // the normed input is not needed any more: its buffer takes the attention's output
+    if (!rc)
+        rc = ck_paged_attention(kv->cache, kv->n_heads, CK_F32, q_dev, H, kv->k_cache_dev, kv->v_cache_dev, kv->table_dev,
+                                kv->table_stride, kv->max_blocks, kv->kv_len_dev, kv->q_start_dev, kv->nreq, ntok,
+                                kv->scale, 1, kv->window, s->w.a, H, nullptr, kv->workspace_dev, kv->workspace_bytes,
+                                stream);
+    if (!rc) rc = ck::launch_q4k_matvec((const uint8_t *)s->wo, s->w.a, s->w.o, H, H, ntok, st);
+    if (!rc)
+        rc = ck_rmsnorm_add(CK_F32, s->w.o, H, CK_F32, h_dev, h_dev, H, s->g_ffn, CK_BF16, s->w.b, H, ntok, H, s->cfg.eps,
+                            stream);
+    if (!rc)
+        rc = ck_moe_layer_bf16(&s->cfg.moe, s->w.b, ntok, s->wg, s->wu, s->wd, s->sg, s->su, s->sd, s->router, s->bias,
+                               s->w.ids, s->w.wts, s->w.counts, s->w.m, s->w.moe_ws, s->w.moe_ws_bytes, stream);
+    if (rc) return rc;
+    const size_t n = (size_t)ntok * H;
+    k_add_bf16<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(h_dev, s->w.m, n);
+    return (int)cudaGetLastError();
+}
+
+int ck_decode_step_capture_kv(ck_decode_step *s, float *h_dev, float *q_dev, float *k_dev, float *v_dev, uint32_t ntok,
+                              const ck_step_kv *kv, void *stream) {
+    if (!s) return CK_EARG;
+    return capture(s, stream, [&] { return ck_decode_step_run_kv(s, h_dev, q_dev, k_dev, v_dev, ntok, kv, stream); });
 }
 
 int ck_decode_step_replay(ck_decode_step *s, void *stream) {

@@ -417,6 +417,33 @@ int ck_paged_attention(const ck_kv_config *cfg, uint32_t n_heads, int io_type, c
  * device-side wait gave up (out is then not valid), else 0. */
 int ck_paged_attention_status(const void *workspace_dev, void *stream);
 
+/* The decode step over a paged cache.  Per token, in one stream:
+ *   a = rmsnorm(h, g_attn); q = Wq a, k = Wk a, v = Wv a; k, v appended at slots;
+ *   o = attention of q over the request's pages (f32 form, causal); h += Wo o;
+ *   b = bf16(rmsnorm(h, g_ffn)); h += ck_moe_layer_bf16(b).
+ * The step's Wq and Wo are Q4_K [hidden x hidden], Wk and Wv [n_kv_heads * head_dim x hidden];
+ * n_heads * head_dim == hidden.  No rotary embedding is applied, as in ck_decode_step_run.  q fp32
+ * [ntok, hidden], k and v fp32 [ntok, n_kv_heads * head_dim] are outputs.  The rows are the plan's: a batch
+ * mixes decodes and chunks freely within max_tokens.  The struct and *cache are read during the call only;
+ * a capture records the addresses in them, so that a plan that advances the same buffers before each
+ * ck_decode_step_replay makes it the next step.  workspace: ck_paged_attention_workspace_bytes. */
+typedef struct {
+    const ck_kv_config *cache;
+    void *k_cache_dev, *v_cache_dev;
+    const int32_t *table_dev;
+    uint64_t table_stride;
+    const int32_t *kv_len_dev, *q_start_dev;
+    const int64_t *slots_dev;
+    uint32_t max_blocks, nreq, n_heads, window;
+    float scale;
+    void *workspace_dev;
+    size_t workspace_bytes;
+} ck_step_kv;
+int ck_decode_step_run_kv(ck_decode_step *step, float *h_dev, float *q_dev, float *k_dev, float *v_dev, uint32_t ntok,
+                          const ck_step_kv *kv, void *stream);
+int ck_decode_step_capture_kv(ck_decode_step *step, float *h_dev, float *q_dev, float *k_dev, float *v_dev, uint32_t ntok,
+                              const ck_step_kv *kv, void *stream);
+
 /* Failure-path self-test (no counterpart in the reference).  Runs the library's bounded device wait
  * on an mbarrier that nothing ever arrives on, with a time limit of limit_ns (1 ns .. 2 s): the wait
  * gives up, writes code 77 to *err_dev (which the caller zeroes first) and the time it waited to
