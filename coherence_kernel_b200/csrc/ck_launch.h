@@ -174,7 +174,7 @@ int launch_rmsnorm_add(int x_type, const void *x, uint64_t x_stride, int res_typ
                        uint64_t res_stride, const float *gain, int out_type, void *out, uint64_t out_stride,
                        uint32_t ntok, uint32_t hidden, float eps, cudaStream_t s);
 // block tables and slot maps from request lengths, and the K/V write (kv_kernels.cu)
-constexpr uint32_t KV_PLAN_MAX_REQUESTS = 16384;  // three running sums per request in shared memory
+constexpr uint32_t KV_PLAN_MAX_REQUESTS = 8192;  // three running sums and two lengths each in shared memory
 struct KvPlanParams {
     const int32_t *len_in, *new_tokens, *count_in;
     int32_t *table, *free_blocks;

@@ -50,53 +50,66 @@ struct ReqPlan {
     int len, rows, have, want;  // want: pages after the call if it is served
     bool fits;                  // its rows and its pages fit the caller's arrays
 };
-CK_DEV ReqPlan req_plan(const KvPlanParams &p, int r, int row_end) {
-    ReqPlan q;
-    const int cap = (int)min((int64_t)p.max_blocks * p.btd.d, (int64_t)SAT);
-    q.len = min(max(p.len_in[r], 0), cap);
-    const int nw = p.new_tokens[r];
-    const int after = (int)min(max((int64_t)q.len + nw, (int64_t)0), (int64_t)SAT);
-    q.rows = max(nw, 0);
-    q.have = (int)p.btd.div((uint32_t)q.len + p.btd.d - 1);
-    q.want = (int)p.btd.div((uint32_t)after + p.btd.d - 1);
-    q.fits = q.rows > 0 && after <= cap && row_end <= (int)p.ntok;
-    return q;
-}
 
-// The request lengths decide everything, so every CTA of the (single) cluster scans all of them --
-// a few loads per thread -- and no CTA waits for another's result.  The sums over the requests
-// (rows, pages needed, pages returned) stay in shared memory, and the rows, the new table entries
-// and the returned pages are each a flat range that the cluster's threads share out evenly, finding
-// an element's request by binary search: one long prompt among a thousand decodes costs no more
-// than its share.  Inputs that alias outputs (len, count) are read before the cluster's barrier and
-// written after it.
+// The request lengths decide everything, so every CTA scans all of them -- a few loads per thread -- and no
+// CTA waits for another's result.  The lengths and the sums over the requests (rows, pages needed, pages
+// returned) stay in shared memory, and the rows, the new table entries and the returned pages are each a
+// flat range that the grid's threads share out evenly, finding an element's request by binary search: one
+// long prompt among a thousand decodes costs no more than its share.
 //
 // Taking a page never waits for a push either: the stack with the returned pages on top is read
 // through the request that returned them, whose own table entries this call does not change.
+//
+// ALIAS: the lengths or the count are updated in place.  The CTAs are then one cluster, whose barrier
+// comes between their reads and the writes.  Bound by latency (launch, the lengths, two scans, one lookup
+// chain per row): 64 decodes 4.5 us, 1000 requests with 31,000 rows 8.3 us on 31 CTAs (15.4 us as one cluster of 8 that
+// read the lengths from memory at each lookup).
+template <bool ALIAS>
 __global__ void __launch_bounds__(PLAN_THREADS) k_kv_plan(const KvPlanParams p) {
     extern __shared__ int sm[];
-    int *row_end = sm, *need_end = sm + p.nreq, *back_end = sm + 2 * p.nreq;
+    const int n = (int)p.nreq;
+    int *row_end = sm, *need_end = sm + n, *back_end = sm + 2 * n, *len_of = sm + 3 * n, *new_of = sm + 4 * n;
     __shared__ Sum3 warp_sum[PLAN_THREADS / 32];
     namespace cg = cooperative_groups;
     grid_dep_trigger_small();
     grid_dep_wait();
-    const int n = (int)p.nreq;
     const int count = min(max(p.count_in[0], 0), (int)p.n_blocks);
+    const int cap = (int)(p.max_blocks * p.btd.d);  // below 2^30
+    const auto req_plan = [&](int r) {
+        ReqPlan q;
+        q.len = len_of[r];
+        const int nw = new_of[r];
+        const int after = (int)min(max((int64_t)q.len + nw, (int64_t)0), (int64_t)SAT);
+        q.rows = max(nw, 0);
+        q.have = (int)p.btd.div((uint32_t)q.len + p.btd.d - 1);
+        q.want = (int)p.btd.div((uint32_t)after + p.btd.d - 1);
+        q.fits = q.rows > 0 && after <= cap && row_end[r] <= (int)p.ntok;
+        return q;
+    };
     Sum3 carry = {0, 0, 0};
     for (int base = 0; base < n; base += PLAN_THREADS) {
         const int r = base + (int)threadIdx.x;
         Sum3 v = {0, 0, 0};
-        if (r < n) v.rows = min(max(p.new_tokens[r], 0), SAT);
-        // rows first: whether a request's rows fit decides whether its pages count
+        if (r < n) {
+            len_of[r] = min(max(p.len_in[r], 0), cap);
+            const int nw = p.new_tokens[r];
+            new_of[r] = nw;
+            v.rows = min(max(nw, 0), SAT);
+            v.back = 0;
+            if (nw < 0) {
+                const int len = len_of[r], keep = max(len + max(nw, -SAT), 0);
+                v.back = (int)(p.btd.div((uint32_t)len + p.btd.d - 1) - p.btd.div((uint32_t)keep + p.btd.d - 1));
+            }
+        }
+        // rows and returned pages first: whether a request's rows fit decides whether the pages it needs count
         for (int pass = 0; pass < 2; ++pass) {
             if (pass == 1) {
-                int need = 0, back = 0;
+                int need = 0;
                 if (r < n) {
-                    const ReqPlan q = req_plan(p, r, row_end[r]);
+                    const ReqPlan q = req_plan(r);
                     if (q.fits) need = max(q.want - q.have, 0);
-                    if (p.new_tokens[r] < 0) back = q.have - q.want;
                 }
-                v = {0, need, back};
+                v = {0, need, 0};
             }
             Sum3 w = warp_scan3(v);
             if ((threadIdx.x & 31) == 31) warp_sum[threadIdx.x >> 5] = w;
@@ -111,11 +124,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_kv_plan(const KvPlanParams p) 
             if (wi == 0) prev = {0, 0, 0};
             w = add3(add3(w, prev), carry);
             if (r < n) {
-                if (pass == 0) row_end[r] = w.rows;
-                else need_end[r] = w.need, back_end[r] = w.back;
+                if (pass == 0) row_end[r] = w.rows, back_end[r] = w.back;
+                else need_end[r] = w.need;
             }
-            if (pass == 0) carry.rows = sat_add(carry.rows, all.rows);
-            else carry = add3(carry, Sum3{0, all.need, all.back});
+            carry = add3(carry, all);
             __syncthreads();
         }
     }
@@ -137,11 +149,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_kv_plan(const KvPlanParams p) 
         if (at < count) return at >= 0 ? p.free_blocks[at] : -1;
         const int i = at - count, r = upper(back_end, n, i);
         if (r >= n) return -1;
-        const ReqPlan q = req_plan(p, r, row_end[r]);
+        const ReqPlan q = req_plan(r);
         return p.table[(uint64_t)r * p.table_stride + q.want + (i - (back_end[r] - (q.have - q.want)))];
     };
-    // every value the writes below depend on that they may overwrite is read before the barrier: the
-    // lengths through req_plan, so each thread's own requests' results are computed here
     const int gt = (int)(blockIdx.x * PLAN_THREADS + threadIdx.x), gn = (int)(gridDim.x * PLAN_THREADS);
 
     // slots and positions of the rows
@@ -151,7 +161,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_kv_plan(const KvPlanParams p) 
         int pos = -1;
         if (t < live) {
             const int r = upper(row_end, n, t);
-            const ReqPlan q = req_plan(p, r, row_end[r]);
+            const ReqPlan q = req_plan(r);
             if (served(q, r)) {
                 pos = q.len + t - (row_end[r] - q.rows);
                 const int b = (int)p.btd.div((uint32_t)pos);
@@ -166,23 +176,22 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_kv_plan(const KvPlanParams p) 
     // new table entries
     for (int k = gt; k < taken; k += gn) {
         const int r = upper(need_end, n, k);
-        const ReqPlan q = req_plan(p, r, row_end[r]);
+        const ReqPlan q = req_plan(r);
         p.table[(uint64_t)r * p.table_stride + q.have + (k - (need_end[r] - (q.want - q.have)))] = page(k);
     }
     // returned pages that nobody took: pushed above the old top
     for (int i = gt; i < top - taken - count; i += gn) {
         const int r = upper(back_end, n, i);
-        const ReqPlan q = req_plan(p, r, row_end[r]);
+        const ReqPlan q = req_plan(r);
         if (count + i < (int)p.n_blocks)
             p.free_blocks[count + i] =
                 p.table[(uint64_t)r * p.table_stride + q.want + (i - (back_end[r] - (q.have - q.want)))];
     }
     for (int r = gt; r <= n; r += gn) p.q_start[r] = r ? min(row_end[r - 1], (int)p.ntok) : 0;
-    // the lengths and the count may be the inputs' own memory: written once every CTA has read them
-    cg::this_cluster().sync();
+    if (ALIAS) cg::this_cluster().sync();  // every CTA has read the lengths and the count
     for (int r = gt; r < n; r += gn) {
-        const ReqPlan q = req_plan(p, r, row_end[r]);
-        const int nw = p.new_tokens[r];
+        const ReqPlan q = req_plan(r);
+        const int nw = new_of[r];
         const bool ok = served(q, r);
         const int after = (int)max((int64_t)q.len + nw, (int64_t)0);
         const int len = nw > 0 && !ok ? q.len : after;
@@ -221,21 +230,27 @@ __global__ void __launch_bounds__(256) k_kv_append(const KvAppendParams p) {
 }  // namespace
 
 int launch_kv_plan(const KvPlanParams &p, cudaStream_t s) {
-    const size_t smem = (size_t)p.nreq * 12;
+    const size_t smem = (size_t)p.nreq * 20;
     static unsigned long long done = 0;
     if (attr_pending(done)) {
-        cudaError_t e = cudaFuncSetAttribute(k_kv_plan, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             KV_PLAN_MAX_REQUESTS * 12);
+        cudaError_t e = cudaFuncSetAttribute(k_kv_plan<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             KV_PLAN_MAX_REQUESTS * 20);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(k_kv_plan<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     KV_PLAN_MAX_REQUESTS * 20);
         if (e != cudaSuccess) return (int)e;
         attr_mark(done);
     }
-    // one cluster: 1 CTA while a thread has at most four rows and requests, else 8
-    const uint32_t ctas = p.ntok <= 4 * PLAN_THREADS && p.nreq <= 4 * PLAN_THREADS ? 1 : 8;
+    // a CTA per 1024 rows or requests; one cluster (of 1, 2, 4 or 8) where the state is updated in place
+    const bool alias = p.len_out == p.len_in || p.count_out == p.count_in;
+    const uint32_t most = p.ntok > p.nreq ? p.ntok : p.nreq, want = (most + PLAN_THREADS - 1) / PLAN_THREADS;
+    uint32_t ctas = want < 1 ? 1 : want < SMS ? want : SMS;
+    if (alias) ctas = want <= 1 ? 1 : want <= 2 ? 2 : want <= 4 ? 4 : 8;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = ctas;
+    attr[1].val.clusterDim.x = alias ? ctas : 1;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
@@ -244,7 +259,7 @@ int launch_kv_plan(const KvPlanParams &p, cudaStream_t s) {
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return (int)cudaLaunchKernelEx(&cfg, k_kv_plan, p);
+    return (int)(alias ? cudaLaunchKernelEx(&cfg, k_kv_plan<true>, p) : cudaLaunchKernelEx(&cfg, k_kv_plan<false>, p));
 }
 
 int launch_kv_append(const KvAppendParams &p, int in_type, cudaStream_t s) {

@@ -195,35 +195,36 @@ def route_dsv4(logits, bias, nused, wscale):
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 
-def _on(device):
-    """(device guard or None, the device's current stream): a guard only where the tensors lie on another
-    device than the current one, which a small call's time cannot hide."""
-    i = device.index
-    guard = None if i is None or i == torch.cuda.current_device() else torch.cuda.device(device)
-    return guard, torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if i is None else i)
+_FN = {}
+_get_device, _get_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 def _call(name, device, *args):
-    """The C call on the device's current stream, appended to the arguments; raises on an error code."""
-    guard, stream = _on(device)
-    fn = getattr(_lib.load(), name)
-    if guard is None:
-        rc = fn(*args, stream)
+    """The C call on the device's current stream, appended to the arguments; raises on an error code.  A
+    device guard only where the tensors lie on another device than the current one: its cost, like
+    that of a Stream object, shows in a small call's time."""
+    fn = _FN.get(name)
+    if fn is None:
+        fn = _FN[name] = getattr(_lib.load(), name)
+    i = device.index
+    if i == _get_device():
+        rc = fn(*args, _get_stream(i))
     else:
-        with guard:
-            rc = fn(*args, stream)
+        with torch.cuda.device(device):
+            rc = fn(*args, _get_stream(i))
     if rc:
         _lib.check(rc, name)
 
 
 def _matrix(t, name, device, shape):
     """The row stride of a CUDA matrix of this shape with contiguous rows, on this device."""
-    if not t.is_cuda or t.device != device or t.dtype not in _FLOATS:
-        raise ValueError(f"{name} must be a CUDA tensor of f32, f16 or bf16 on {device}")
-    st = t.stride()
-    if t.shape != shape or (st[1] != 1 and shape[1] > 1) or (shape[0] > 1 and st[0] < shape[1]):
-        raise ValueError(f"{name} must be {tuple(shape)} with contiguous rows")
-    return st[0] if shape[0] > 1 else shape[1]
+    if t.shape != shape or t.device != device or t.dtype not in _FLOATS:
+        raise ValueError(f"{name} must be {list(shape)} of f32, f16 or bf16 on {device}")
+    row, col = t.stride()
+    n, width = shape
+    if (col != 1 and width > 1) or (n > 1 and row < width):
+        raise ValueError(f"{name}'s rows must be contiguous and apart")
+    return row if n > 1 else width
 
 
 def rmsnorm_add(x, residual, gain, eps, out_dtype=None, out=None, residual_out=None):
@@ -232,8 +233,8 @@ def rmsnorm_add(x, residual, gain, eps, out_dtype=None, out=None, residual_out=N
     s is stored to residual_out, by default the residual itself.  out_dtype: f32, f16, bf16 (default x's)
     or "q8_0", which returns the rows' GGUF blocks as uint8 [ntok, hidden // 32 * 34]."""
     shape, dev = x.shape, x.device
-    if len(shape) != 2:
-        raise ValueError("x must be [ntok, hidden]")
+    if len(shape) != 2 or dev.type != "cuda":
+        raise ValueError("x must be a CUDA tensor [ntok, hidden]")
     ntok, hidden = shape
     xs = _matrix(x, "x", dev, shape)
     rs, rt, rp, rop = 0, 0, None, None
@@ -246,7 +247,8 @@ def rmsnorm_add(x, residual, gain, eps, out_dtype=None, out=None, residual_out=N
             rop = residual_out.data_ptr()
     elif residual_out is not None:
         raise ValueError("residual_out without a residual")
-    _dev(gain, "gain", torch.float32, hidden)
+    if gain.dtype is not torch.float32 or gain.device != dev or gain.numel() < hidden or not gain.is_contiguous():
+        raise ValueError(f"gain must be a contiguous f32 tensor of {hidden} elements on {dev}")
     if out_dtype is None:
         out_dtype = out.dtype if out is not None else x.dtype
     ot = TYPE_NUMBERS.get(out_dtype)
@@ -255,16 +257,18 @@ def rmsnorm_add(x, residual, gain, eps, out_dtype=None, out=None, residual_out=N
     if ot == 8:
         if out is None:
             out = torch.empty((ntok, hidden // 32 * Q8_0_BLOCK_BYTES), dtype=torch.uint8, device=dev)
+        elif out.device != dev:
+            raise ValueError(f"out must be on {dev}")
         _dev(out, "out", torch.uint8, ntok * (hidden // 32) * Q8_0_BLOCK_BYTES)
         os_ = 0
     else:
         if out is None:
             out = torch.empty(shape, dtype=out_dtype, device=dev)
+            os_ = hidden
         elif out.dtype != out_dtype:
             raise ValueError(f"out has dtype {out.dtype}, expected {out_dtype}")
-        os_ = _matrix(out, "out", dev, shape)
-    if gain.device != dev or out.device != dev:
-        raise ValueError("x, gain and out must be on one device")
+        else:
+            os_ = _matrix(out, "out", dev, shape)
     _call("ck_rmsnorm_add", dev, TYPE_NUMBERS[x.dtype], x.data_ptr(), xs, rt, rp, rop, rs, gain.data_ptr(), ot,
           out.data_ptr(), os_, ntok, hidden, eps)
     return out

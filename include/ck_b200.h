@@ -365,9 +365,9 @@ int ck_rmsnorm_add(int x_type, const void *x_dev, uint64_t x_stride, int res_typ
  * Outputs: len_out[r] the tokens held; kv_len[r] the tokens its new rows attend over (len_out, but 0
  * where it has rows and is not served); q_start[nreq + 1] the first row of each request (at most ntok);
  * for every row t < ntok its slot and position, -1 for rows of requests not served and rows past the
- * last; *count_out the free pages.  len_out may be len_in and count_out count_in: a captured graph then
- * advances the state at each replay.  Free list entries outside the cache give slots of -1.
- * nreq <= 16384, ntok < 2^30, max_blocks * block_tokens < 2^30, n_blocks * block_tokens < 2^31;
+ * last; *count_out the free pages.  len_out may be len_in and count_out count_in (the same addresses, not
+ * shifted ones): a captured graph then advances the state at each replay.  Free list entries outside the cache give slots of -1.
+ * nreq <= 8192, ntok < 2^30, max_blocks * block_tokens < 2^30, n_blocks * block_tokens < 2^31;
  * free_blocks holds n_blocks entries. */
 int ck_kv_plan(const int32_t *len_in_dev, const int32_t *new_tokens_dev, uint32_t nreq, int32_t *table_dev,
                uint64_t table_stride, uint32_t max_blocks, int32_t *free_blocks_dev, const int32_t *count_in_dev,

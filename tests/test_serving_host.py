@@ -42,7 +42,7 @@ def plan(L, **kw):
 @pytest.mark.parametrize("kw,rc", [
     (dict(ln=None), EARG), (dict(new=None), EARG), (dict(table=None), EARG), (dict(free=None), EARG),
     (dict(ci=None), EARG), (dict(lo=None), EARG), (dict(co=None), EARG), (dict(kl=None), EARG), (dict(qs=None), EARG),
-    (dict(sl=None), EARG), (dict(pos=None), EARG), (dict(ts=7), EARG), (dict(nreq=16385), ESHAPE),
+    (dict(sl=None), EARG), (dict(pos=None), EARG), (dict(ts=7), EARG), (dict(nreq=8193), ESHAPE),
     (dict(ntok=1 << 30), ESHAPE), (dict(bt=0), ESHAPE), (dict(mb=0, ts=0), ESHAPE), (dict(nb=0), ESHAPE),
     (dict(mb=1 << 27, ts=1 << 27), ESHAPE), (dict(nb=1 << 27), ESHAPE)])
 def test_plan_refusals(cuda_lib, kw, rc):
