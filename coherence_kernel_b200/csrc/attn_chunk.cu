@@ -144,6 +144,11 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     const uint32_t sbase = smem_u32(smem);
     const int wg = threadIdx.x >> 7, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     grid_dep_trigger_small();
+    if (TMA && threadIdx.x == 0) {
+        prefetch_tmap(&kmap);
+        prefetch_tmap(&vmap);
+        if (qbox) prefetch_tmap(&qmap);
+    }
     grid_dep_wait();
     if (blockIdx.x == 0 && threadIdx.x == 0) *p.err = 0;
     long long U;
@@ -522,12 +527,15 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                 for (int b = 0; b < 4; ++b) tmem_ld32(s_at + b * 32, s[b]);
                 tmem_ld_wait();
                 if (j0 < all_lo || j0 + KC > all_hi) {
-                    const int a = lo - j0, z = hi - j0;
 #pragma unroll
-                    for (int b = 0; b < 4; ++b)
+                    for (int b = 0; b < 4; ++b) {
+                        // bit x: the row sees key j0 + 32 b + x
+                        const int a = min(max(lo - j0 - b * 32, 0), 32), z = min(max(hi - j0 - b * 32, 0), 32);
+                        const uint32_t see = (uint32_t)((1ull << z) - 1) & ~(uint32_t)((1ull << a) - 1);
 #pragma unroll
                         for (int x = 0; x < 32; ++x)
-                            if (b * 32 + x < a || b * 32 + x >= z) s[b][x] = 0xFF800000u;  // -infinity
+                            if (!(see & (1u << x))) s[b][x] = 0xFF800000u;  // -infinity
+                    }
                 }
                 float mx[4];
 #pragma unroll

@@ -77,10 +77,10 @@ struct Sched {
         if (r < (int)p.nreq) q = load_req(p, r);
         const int nt = r < (int)p.nreq ? tiles(p, q) : 0;
         long long n = 0;
-        if (nt <= 4)
+        if (nt <= 8)
             for (int t = 0; t < nt; ++t) n += tile_geo<TR, KC, ALIGN>(p, q, t).nch + EXTRA;
         // requests of many tiles: the warp's lanes share them out
-        for (uint32_t todo = __ballot_sync(0xffffffffu, nt > 4); todo; todo &= todo - 1) {
+        for (uint32_t todo = __ballot_sync(0xffffffffu, nt > 8); todo; todo &= todo - 1) {
             const int src = __ffs(todo) - 1;
             const Req w = {0, __shfl_sync(0xffffffffu, q.nq, src), __shfl_sync(0xffffffffu, q.kl, src)};
             const int wt = __shfl_sync(0xffffffffu, nt, src);
