@@ -668,14 +668,19 @@ int ck_paged_attention(const ck_kv_config *c, uint32_t n_heads, int io_type, con
     p.causal = causal;
     p.io_type = io_type;
     p.cache_type = (int)c->cache_type;
-    // Requests of many rows take the chunk form, the others the few-row form in a launch of its own.  A batch
+    // Requests of many rows take the chunk form, the others the few-row form, in launches of its own.  A batch
     // with no more rows than requests is a decode step, and its requests have one row each (or padding): only
     // the few-row form is launched, unless a single token's heads already fill a chunk tile's threshold.
     const bool decode = ntok <= nreq && p.gd.d < ck::ATTN_CHUNK_ROWS;
     const bool chunk = !decode && ck::attn_chunk_ok_types(io_type, (int)c->cache_type, c->head_dim) &&
                        (uint64_t)ntok * p.gd.d >= ck::ATTN_CHUNK_ROWS;
-    // of a single request the chunk form takes what it gets, in one launch
-    p.row_split = !chunk ? ck::ATTN_NO_CHUNK : nreq == 1 ? 0 : ck::ATTN_CHUNK_ROWS;
+    // The chunk form streams a decode row's keys at three quarters of the few-row form's rate (64 ragged decodes
+    // of up to 8192 tokens: 257 against 193 us), and a second pair of launches costs 14 us (17 requests, chunks and
+    // decodes of up to 5000 tokens: 69 against 55 us).  So it takes every request of a batch whose keys, at the
+    // most the tables can name, stream in less than about four times that.
+    const bool small = (uint64_t)nreq * max_blocks * c->block_tokens * c->n_kv_heads * c->head_dim * 4 < 360ull << 20;
+    const bool all = nreq == 1 || small;
+    p.row_split = !chunk ? ck::ATTN_NO_CHUNK : all ? 0 : ck::ATTN_CHUNK_ROWS;
     uint8_t *at = (uint8_t *)ws + 256;  // after the error word: each form's cuts, then its parts
     const auto take = [&](size_t bytes) { uint8_t *b = at; at += al(bytes); return b; };
     p.cuts = (ck::AttnCuts *)take(sizeof(ck::AttnCuts));
@@ -685,7 +690,7 @@ int ck_paged_attention(const ck_kv_config *c, uint32_t n_heads, int io_type, con
         g.cuts = (ck::AttnCuts *)take(sizeof(ck::AttnCuts));
         g.part_o = (float *)take(ck::attn_chunk_workspace_bytes(c->head_dim));
         rc = ck::launch_attn_chunk(g, S(s));
-        if (rc || nreq == 1) return fail(rc, "ck_paged_attention");
+        if (rc || all) return fail(rc, "ck_paged_attention");
     }
     return fail(ck::launch_attn_few(p, S(s)), "ck_paged_attention");
 }

@@ -307,6 +307,16 @@ def test_attention_chunk_form_many_heads_over_one():
     check_attn(attn_case(3, [(300, 1), (77, 1), (1, 1), (513, 2)], 128, 1, 128, 16, BF16, BF16))
 
 
+def test_attention_both_forms_in_one_call():
+    """A table wide enough that decode rows and chunks take their own launches (64 or more rows the chunk form)."""
+    lens = [(300, 1), (500, 130), (77, 3), (20, 20), (400, 64), (1, 1), (0, 0), (3000, 1)]
+    q, k, v, table, kl, starts = attn_case(5, lens, 4, 2, 128, 16, BF16, BF16)
+    wide = 8192 * 16 // 16  # 8 requests x 131072 tokens x 2 heads x 128 x 4 bytes: past the one-launch rule
+    table = [row + [-1] * (wide - len(row)) for row in table]
+    check_attn((q, k, v, table, kl, starts), pad=3)
+    check_attn((q, k, v, table, kl, starts), window=100)
+
+
 def test_attention_chunk_form_growing_scores():
     """Scores that keep growing along the keys: every unit moves the running maximum past the rescaling step."""
     q, k, v, table, kl, starts = attn_case(3, [(1400, 150)], 2, 2, 64, 16, F16, F16)
