@@ -5,10 +5,12 @@
 // SM of four warpgroups:
 //   0, 1  softmax: each owns 128 rows, a thread one row.  Reads its scores from tensor memory (all 128 of
 //         a unit in registers), masks, keeps maximum and sum, and writes P as bf16 / f16 pairs over the
-//         scores it came from -- the A operand of the second product never leaves tensor memory
-//   2     loader: K and V rows by 16-byte asynchronous copies (each row's page looked up by one lane a unit
-//         ahead, so any page size and stride works) into a ring of four 128-key tiles in the 128-byte-swizzle
-//         layout; the query tile at each item's start
+//         scores it came from -- the A operand of the second product never leaves tensor memory.  P is handed over
+//         in two halves, so that the product over the first runs beside the second's exponentials
+//   2     loader: one warp issues TMA loads of K and V (a box of up to 64 tokens of a page, its page looked up by a
+//         lane a unit ahead) and of the queries into a ring of four 128-key tiles, 128-byte swizzle; the others clean
+//         V tiles on the edge of the mask.  Pages that hold no multiple of 8 tokens, and query groups that
+//         are no power of two, come by 16-byte asynchronous copies instead
 //   3     one warp issues the products: S_t = Q_t K^T (both operands in shared memory) and
 //         O_t += P_t V (P in tensor memory, V as an N-major B operand straight from its row layout)
 // Tensor memory: S_0 S_1 O_0 O_1, 128 columns each.  The issue order PV_0(i) S_0(i+1) PV_1(i) S_1(i+1) keeps the
@@ -20,8 +22,13 @@
 // round trip of O through registers.  P is rounded once to the cache's type (half an ulp of each weight,
 // below the output's own rounding); scores, sums and O are fp32.
 //
-// Bound: the tensor core (4 x 128 x 128 x 128 multiply-adds, 2048 cycles per unit) and the exponentials (2 x 128
-// x 128 at 16 per cycle: 2048 cycles) alike.
+// Bounds per unit: the tensor core (4 x 128 x 128 x 128 multiply-adds, 2048 cycles), the exponentials (2 x 128 x 128 at 16
+// per cycle, 2048 cycles) and the tiles' way from L2 (64 KB at about 26 bytes per cycle, 2500 cycles) are close to
+// each other, and the chain scores - softmax - product of a half leaves gaps between them: about 4100 cycles.
+// 2048 new tokens of 8192, 32 heads over 8 of 128: 241 us, 998 TFLOP/s, 61% of the measured bf16 GEMM rate (tensor pipe 48%
+// active, special-function unit 48%).  Tried and slower: steps of 64 keys with their own score columns (271 us: an
+// N = 64 product of two shared-memory operands waits for shared memory), two threads per row (253), a
+// polynomial for a share of the exponentials (262 to 349, the share from 1/8 to 1/2).
 #include "attn_sched.cuh"
 
 namespace ck {
@@ -719,8 +726,8 @@ int launch(AttnParams p, int box, cudaStream_t s) {
     return (int)e;
 }
 
-// TMA where the pages allow it (2048 new tokens of 8192, pages of 16: 16-byte copies keep a loader at 21 bytes per
-// cycle and SM, about 1500 cycles a tile, and bound the kernel), else the copies.
+// TMA where the pages allow it, else the copies: 16-byte copies are issued at 21 bytes per cycle and SM (about 1500 cycles
+// a tile), close to the whole unit's time, and take four warps.
 template <int TYPE, int DP>
 int launch_pages(const AttnParams &p, cudaStream_t s) {
     const int box = kv_box(p.btd.d, 64);
