@@ -330,9 +330,19 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                 // the queries, and the V tiles to clean
                 const int me = threadIdx.x - 288;  // 0 .. 95
                 uint32_t raw_parity = 0;           // a bit per stage
+                // the three warps go on or give up together: they meet at a barrier below
+                const auto together = [](bool ok) -> bool {
+                    uint32_t r;
+                    asm volatile(
+                        "{\n .reg .pred a, b;\n setp.ne.u32 a, %1, 0;\n barrier.cta.red.and.pred b, 2, 96, a;\n selp.u32 %0, 1, 0, b;\n}"
+                        : "=r"(r)
+                        : "r"((uint32_t)ok)
+                        : "memory");
+                    return r != 0;
+                };
                 do {
                     if (!qbox) {
-                        ok = room(&bar->q_empty, (item & 1) ^ 1);
+                        ok = together(mbar_wait_short(&bar->q_empty, (item & 1) ^ 1, p.err, 30));
                         if (!ok) break;
                         for (int b = w - 1; b < TR / 32; b += 3) copy_queries(b);
                         hand_over(&bar->q_full);
@@ -347,7 +357,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                         const int j0 = it.g.lo + c * KC;
                         if (j0 >= all_lo && j0 + KC <= all_hi) continue;
                         const uint32_t st = (e + 1) % NS;
-                        ok = __all_sync(0xffffffffu, mbar_wait_short(&bar->raw[st], raw_parity >> st & 1, p.err, 41));
+                        ok = together(mbar_wait_short(&bar->raw[st], raw_parity >> st & 1, p.err, 41));
                         if (!ok) break;
                         raw_parity ^= 1u << st;
                         clean(sbase + F::RING_OFF + st * F::TILE, item, KC, me, 96, it.g.hi - j0);
@@ -717,10 +727,11 @@ int launch(AttnParams p, int box, cudaStream_t s) {
     CUtensorMap kmap = {}, vmap = {}, qmap = {};
     // queries by TMA too where a 128-row tile is whole tokens of the group's heads (powers of two up to 128)
     const uint32_t group = p.gd.d;
-    const int qbox = TMA && group <= 128 && (group & (group - 1)) == 0 ? 128 / (int)group : 0;
-    if (qbox && make_q_map(&qmap, p, qbox)) return CK_ERR_ARG;
+    int qbox = TMA && group <= 128 && (group & (group - 1)) == 0 ? 128 / (int)group : 0;
+    if (qbox && make_q_map(&qmap, p, qbox)) qbox = 0;
     cudaError_t e;
-    if (TMA && (make_kv_map(&kmap, p.k, p, box) || make_kv_map(&vmap, p.v, p, box))) return CK_ERR_ARG;
+    if (TMA && (make_kv_map(&kmap, p.k, p, box) || make_kv_map(&vmap, p.v, p, box)))
+        return launch<TYPE, DP, false>(p, 0, s);  // strides that no tensor map takes
     e = launch_pdl(k_attn_chunk<TYPE, DP, TMA>, dim3(grid), dim3(NTHREADS), F::SMEM, s, p, kmap, vmap, qmap, box, qbox);
     if (e == cudaSuccess) e = launch_pdl(k_attn_join_chunk<DP>, dim3(grid - 1, DP / 8), dim3(TR), 0, s, p);
     return (int)e;

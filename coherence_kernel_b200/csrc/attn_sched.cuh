@@ -84,9 +84,9 @@ struct Sched {
             const int src = __ffs(todo) - 1;
             const Req w = {0, __shfl_sync(0xffffffffu, q.nq, src), __shfl_sync(0xffffffffu, q.kl, src)};
             const int wt = __shfl_sync(0xffffffffu, nt, src);
-            int part = 0;
+            long long part = 0;
             for (int t = threadIdx.x & 31; t < wt; t += 32) part += tile_geo<TR, KC, ALIGN>(p, w, t).nch + EXTRA;
-            part = __reduce_add_sync(0xffffffffu, part);
+            for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
             if ((int)(threadIdx.x & 31) == src) n = part;
         }
         return n * (int)p.n_kv;
@@ -149,7 +149,7 @@ struct Sched {
         if (u >= ex && u < ex + mine) {  // one thread: its request holds the unit
             sh.before = u - ex;
             sh.req = q;
-            if (tiles(p, q) == 1) place(p, sh, q, 0, tile_geo<TR, KC, ALIGN>(p, q, 0), (int)(u - ex));
+            if (tiles(p, q) == 1) place(p, sh, q, 0, tile_geo<TR, KC, ALIGN>(p, q, 0), u - ex);
         }
         __syncthreads();
         const int nt = tiles(p, sh.req);
@@ -170,7 +170,7 @@ struct Sched {
                     }
                     const long long tot = __shfl_sync(0xffffffffu, s, 31);
                     if (v < tot) {
-                        if (v >= s - m && v < s) place(p, sh, q, t, g, (int)(v - (s - m)));
+                        if (v >= s - m && v < s) place(p, sh, q, t, g, v - (s - m));
                         break;
                     }
                     v -= tot;
@@ -182,10 +182,11 @@ struct Sched {
         geo = sh.geo;
         return true;
     }
-    static CK_DEV void place(const AttnParams &p, Shared &sh, const Req &q, int t, const Geo &g, int in) {
+    static CK_DEV void place(const AttnParams &p, Shared &sh, const Req &q, int t, const Geo &g, long long in) {
+        const uint32_t per = (uint32_t)(g.nch + EXTRA);
         sh.pos.t = t;
-        sh.pos.h = in / (g.nch + EXTRA);
-        sh.pos.c = in - sh.pos.h * (g.nch + EXTRA);
+        sh.pos.h = in < 1ll << 32 ? (int)((uint32_t)in / per) : (int)(in / per);
+        sh.pos.c = (int)(in - (long long)sh.pos.h * per);
         sh.geo = g;
     }
 

@@ -155,6 +155,8 @@ class PagedAttention:
         nreq, max_blocks = table.shape
         if ntok > self.max_tokens or nreq > self.max_requests:
             raise ValueError("more rows or requests than this object was made for")
+        if window < 0:
+            raise ValueError("window must not be negative")
         shape = (ntok, heads, dim)
         qs = _rows3(q, "q", shape, (k_cache.dtype, torch.float32), dev)
         if out is None:
@@ -178,7 +180,8 @@ class PagedAttention:
 
     def status(self):
         """Synchronize and raise if a device-side wait of the last call gave up."""
-        _lib.check(_lib.load().ck_paged_attention_status(_ptr(self.ws), _stream()), "ck_paged_attention_status")
+        with torch.cuda.device(self.ws.device):
+            _lib.check(_lib.load().ck_paged_attention_status(_ptr(self.ws), _stream()), "ck_paged_attention_status")
 
 
 class PagedKV:

@@ -366,7 +366,8 @@ int ck_rmsnorm_add(int x_type, const void *x_dev, uint64_t x_stride, int res_typ
  * where it has rows and is not served); q_start[nreq + 1] the first row of each request (at most ntok);
  * for every row t < ntok its slot and position, -1 for rows of requests not served and rows past the
  * last; *count_out the free pages.  len_out may be len_in and count_out count_in (the same addresses, not
- * shifted ones): a captured graph then advances the state at each replay.  Free list entries outside the cache give slots of -1.
+ * shifted ones): a captured graph then advances the state at each replay.  No other output may overlap an
+ * input, but for the table and free_blocks, which are updated.  Free list entries outside the cache give slots of -1.
  * nreq <= 8192, ntok < 2^30, max_blocks * block_tokens < 2^30, n_blocks * block_tokens < 2^31;
  * free_blocks holds n_blocks entries. */
 int ck_kv_plan(const int32_t *len_in_dev, const int32_t *new_tokens_dev, uint32_t nreq, int32_t *table_dev,
@@ -394,7 +395,7 @@ int ck_kv_append(const ck_kv_config *cfg, int in_type, const void *k_dev, uint64
 
 /* Attention of each request's new tokens over its cached ones (the new ones among them: append first).
  * Request r's rows are q[q_start[r] .. q_start[r + 1]), its keys the cache's positions
- * 0 .. kv_len[r] - 1 through its table row; the last row is at position kv_len[r] - 1, the row before it
+ * 0 .. kv_len[r] - 1 through its table row (out must not overlap q); the last row is at position kv_len[r] - 1, the row before it
  * one earlier.  A row sees the positions up to its own (causal != 0) or all of them, and of those the last
  * `window` up to its own (window 0: no bound).
  *   out[t, h] = sum_j p_j V[j, h'] / sum_j p_j,  p_j = exp(scale q[t, h] . K[j, h']),  h' = h / (n_heads / n_kv_heads)

@@ -307,6 +307,76 @@ def test_attention_chunk_form_many_heads_over_one():
     check_attn(attn_case(3, [(300, 1), (77, 1), (1, 1), (513, 2)], 128, 1, 128, 16, BF16, BF16))
 
 
+@pytest.mark.parametrize("group", [1, 3, 4])
+def test_attention_chunk_form_head_major_and_odd_groups(group):
+    check_attn(attn_case(8, [(270, 150), (333, 90)], 2 * group, 2, 64, 16, BF16, BF16, head_major=True))
+    check_attn(attn_case(8, [(270, 150), (333, 90)], 2 * group, 2, 128, 12, F16, F16, head_major=True))
+
+
+def test_attention_rows_are_independent():
+    """A NaN query row reaches no other row, and repeated calls give the same bits."""
+    for lens, io in (([(200, 150), (90, 5)], BF16), ([(200, 15), (90, 5)], F32), ([(900, 1)] * 9, BF16)):
+        case = attn_case(5, lens, 4, 2, 64, 16, BF16, io)
+        clean, _ = run_attn(*case, 0.125)
+        q = case[0].clone()
+        q[3, 1] = math.nan
+        out, _ = run_attn(q, *case[1:], 0.125)
+        assert torch.isnan(out[3, 1]).all()
+        keep = torch.ones(q.shape[:2], dtype=torch.bool)
+        keep[3, 1] = False
+        assert torch.equal(out[keep], clean[keep])
+        for _ in range(3):
+            assert torch.equal(run_attn(*case, 0.125)[0], clean)
+
+
+def test_attention_on_two_streams_at_once():
+    i = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    cases = [attn_case(1, [(700, 300), (90, 1)], 4, 2, 128, 16, BF16, BF16),
+             attn_case(2, [(3000, 1)] * 5, 8, 2, 128, 16, BF16, BF16)]
+    want = [run_attn(*c, 0.1)[0] for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    objs = [kv.PagedAttention(c[0].shape[1], 2, 128, c[0].shape[0], len(c[4])) for c in cases]
+    args = [(c[0].cuda(), c[1].cuda(), c[2].cuda(), i(c[3]), i(c[4]), i(c[5])) for c in cases]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(10):
+        for n, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs[n].append(objs[n](*args[n], 0.1))
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert all(torch.equal(x.cpu(), w) for x in o)
+
+
+def test_cache_past_32_bit_offsets():
+    """Pages whose element offsets pass 2^31 and 2^32 bytes: append and both attention forms."""
+    n_blocks, bt, kvh, dim = 140000, 16, 8, 128
+    big = [torch.zeros((n_blocks, bt, kvh, dim), dtype=BF16, device="cuda") for _ in range(2)]
+    g = gen(3)
+    lens = [(150, 100), (40, 1)]
+    pages = [n_blocks - 1 - 3 * b for b in range(10)] + [131072, 70000, 65537]
+    table = [pages[:10], pages[10:] + [0] * 7]
+    rows = [torch.randn(190, kvh, dim, generator=g).to(BF16) for _ in range(2)]
+    slots = torch.tensor([table[0][p // bt] * bt + p % bt for p in range(150)] +
+                         [table[1][p // bt] * bt + p % bt for p in range(40)]).cuda()
+    kv.append(rows[0].cuda(), rows[1].cuda(), big[0], big[1], slots)
+    small = [torch.zeros((13, bt, kvh, dim), dtype=BF16) for _ in range(2)]
+    order = {p: n for n, p in enumerate(pages)}
+    for x, r in zip(small, rows):
+        for t, s in enumerate(slots.tolist()):
+            x[order[s // bt], s % bt] = r[t]
+    for x, y in zip(big, small):
+        assert torch.equal(x[torch.tensor(pages).cuda()].cpu(), y)
+    i = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    for io in (BF16, F32):
+        q = torch.randn(101, 16, dim, generator=g).to(io)
+        want, _, spread, smax = ref.attention(q, small[0], small[1], [list(range(10)), [10, 11, 12] + [0] * 7], [150, 40],
+                                              [0, 100, 101], 0.1)
+        at = kv.PagedAttention(16, kvh, dim, 101, 2)
+        out = at(q.cuda(), big[0], big[1], i(table), i([150, 40]), i([0, 100, 101]), 0.1).cpu().double()
+        assert ((out - want).abs() <= ref.attention_bound(want, spread, smax, dim, 150, io, BF16)).all()
+
+
 def test_attention_both_forms_in_one_call():
     """A table wide enough that decode rows and chunks take their own launches (64 or more rows the chunk form)."""
     lens = [(300, 1), (500, 130), (77, 3), (20, 20), (400, 64), (1, 1), (0, 0), (3000, 1)]
