@@ -600,7 +600,7 @@ int ck_kv_append(const ck_kv_config *c, int in_type, const void *k, uint64_t k_s
 size_t ck_paged_attention_workspace_bytes(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim) {
     if (n_heads == 0 || n_kv_heads == 0 || n_heads % n_kv_heads || head_dim == 0 || head_dim % 8 || head_dim > 256)
         return 0;
-    return 256 + 2 * al(sizeof(ck::AttnCuts)) + al(ck::attn_few_workspace_bytes(head_dim)) +
+    return 256 + al(ck::ATTN_MAX_CTAS * 4) + al(sizeof(ck::AttnCuts)) + al(ck::attn_few_workspace_bytes(head_dim)) +
            al(ck::attn_chunk_workspace_bytes(head_dim));
 }
 
@@ -675,15 +675,15 @@ int ck_paged_attention(const ck_kv_config *c, uint32_t n_heads, int io_type, con
     const bool chunk = !decode && ck::attn_chunk_ok_types(io_type, (int)c->cache_type, c->head_dim) &&
                        (uint64_t)ntok * p.gd.d >= ck::ATTN_CHUNK_ROWS;
     // The chunk form streams a decode row's keys at three quarters of the few-row form's rate (64 ragged decodes
-    // of up to 8192 tokens: 257 against 193 us), and a second pair of launches costs 14 us (17 requests, chunks and
+    // of up to 8192 tokens: 257 against 193 us), and the few-row form beside it costs 14 us (17 requests, chunks and
     // decodes of up to 5000 tokens: 69 against 55 us).  So it takes every request of a batch whose keys, at the
     // most the tables can name, stream in less than about four times that.
     const bool small = (uint64_t)nreq * max_blocks * c->block_tokens * c->n_kv_heads * c->head_dim * 4 < 360ull << 20;
     const bool all = nreq == 1 || small;
     p.row_split = !chunk ? ck::ATTN_NO_CHUNK : all ? 0 : ck::ATTN_CHUNK_ROWS;
-    uint8_t *at = (uint8_t *)ws + 256;  // after the error word: each form's cuts, then its parts
+    uint8_t *at = (uint8_t *)ws + 256;  // after the error word: each form's arrival counts or cuts, and its parts
     const auto take = [&](size_t bytes) { uint8_t *b = at; at += al(bytes); return b; };
-    p.cuts = (ck::AttnCuts *)take(sizeof(ck::AttnCuts));
+    p.arrived = (int *)take(ck::ATTN_MAX_CTAS * 4);
     p.part_o = (float *)take(ck::attn_few_workspace_bytes(c->head_dim));
     if (chunk) {
         ck::AttnParams g = p;

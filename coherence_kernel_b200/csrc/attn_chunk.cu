@@ -684,7 +684,7 @@ template <int DP>
 __global__ void __launch_bounds__(TR) k_attn_join_chunk(const __grid_constant__ AttnParams p) {
     grid_dep_trigger_small();
     grid_dep_wait();
-    Joint jt;
+    Cut jt;
     const int d = (int)blockIdx.y * 8;
     if (d >= (int)p.head_dim || !find_joint<S>(p, (int)blockIdx.x + 1, jt)) return;
     const Req q = load_req(p, jt.at.r);

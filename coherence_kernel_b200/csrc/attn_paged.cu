@@ -1,5 +1,5 @@
 // attn_paged.cu -- attention of few new tokens per request over a paged K/V cache (decode steps,
-// short drafts, and every form the chunk kernel does not take), and the joining of partial results.
+// short drafts, and every form the chunk kernel does not take).
 //
 //   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale q_i . k_j - m_i),  j over the visible keys
 //
@@ -101,6 +101,48 @@ CK_DEV uint32_t finite2(uint32_t w, bool &bad) {
     return (l ? 0u : w & 0xFFFFu) | (h ? 0u : w & 0xFFFF0000u);
 }
 
+// Joins the parts of an item that spans CTAs, in their order: a thread owns four neighbouring columns of a row and
+// carries the running maximum and sum over the parts, whose loads depend on nothing.
+template <int DP>
+CK_DEV void join_parts(const AttnParams &p, const S::Joint &jt, const Pos &at, const Req &q, int rows) {
+    constexpr int COLS = DP / 4;
+    for (int i = threadIdx.x; i < rows * COLS; i += WARPS * 32) {
+        const int r = i / COLS, col = i % COLS * 4;
+        float m = -INFINITY, l = 0.0f;
+        float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll 8
+        for (int k = 0; k < jt.n; ++k) {
+            const size_t s = jt.slot(k) * TR + r;
+            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p.part_ml + s * 2));
+            const float4 v = __ldcg(reinterpret_cast<const float4 *>(p.part_o + s * DP + col));
+            const float mn = fmaxf(m, ml.x), ref = mn == -INFINITY ? 0.0f : mn;
+            const float a = ex2(m - ref), w = ex2(ml.x - ref);
+            m = mn;
+            l = l * a + w * ml.y;
+            o.x = o.x * a + w * v.x;
+            o.y = o.y * a + w * v.y;
+            o.z = o.z * a + w * v.z;
+            o.w = o.w * a + w * v.w;
+        }
+        const bool some = l > 0.0f || l != l;
+        const float inv = some ? 1.0f / l : 0.0f;
+        const int row = at.t * TR + r;
+        const uint32_t tok = p.gd.div((uint32_t)row);
+        const uint32_t head = at.h * p.gd.d + (row - tok * p.gd.d);
+        if (col < (int)p.head_dim) {
+            const uint64_t e = (uint64_t)(q.q0 + tok) * p.out_stride + (uint64_t)head * p.head_dim + col;
+            if (p.io_type == T_F32)
+                *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + e) =
+                    make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+            else
+                *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + e) =
+                    make_uint2(pack2(p.io_type, o.x * inv, o.y * inv), pack2(p.io_type, o.z * inv, o.w * inv));
+        }
+        if (p.lse && col == 0)
+            p.lse[(uint64_t)(q.q0 + tok) * (p.n_kv * p.gd.d) + head] = some ? (m + log2f(l)) * LN2 : -INFINITY;
+    }
+}
+
 template <int TYPE, int DP, int TERMS>
 __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(const __grid_constant__ AttnParams p) {
     using F = Few<DP, TERMS>;
@@ -108,6 +150,7 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ typename S::Shared sh;
     __shared__ float row_scale[TR], wm[WARPS][TR], wl[WARPS][TR];
+    __shared__ int last_part;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t ring = smem_u32(smem) + warp * NS * F::STAGE, qs = smem_u32(smem) + F::RING;
     float *osum = reinterpret_cast<float *>(smem + F::RING);
@@ -118,12 +161,11 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
     int C;
     Pos pos;
     Geo geo;
-    const bool part = S::find(p, sh, (int)gridDim.x, (int)blockIdx.x, U, C, pos, geo);
-    S::leave_cut(p, U, C, pos, geo);
-    if (!part) return;
-    const int n = (int)(S::start(U, C, blockIdx.x + 1) - S::start(U, C, blockIdx.x));
+    if (!S::find(p, sh, (int)gridDim.x, (int)blockIdx.x, U, C, pos, geo)) return;
+    const long long u0 = S::start(U, C, blockIdx.x);
+    const int n = (int)(S::start(U, C, blockIdx.x + 1) - u0);
     typename S::Items use, fill;
-    if (!use.set(p, sh, n)) return;
+    if (!use.set(p, sh, n, u0)) return;
     fill = use;
     int fill_c = fill.c0;
     bool to_fill = true;
@@ -411,78 +453,27 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
                     }
                 }
             }
+            if (!whole) {
+                // the part is out; whoever brings the item's last one joins them all
+                const typename S::Joint jt = S::joint(use, U, C);
+                __threadfence();
+                __syncthreads();
+                if (threadIdx.x == 0) {
+                    const bool last = atomicAdd(p.arrived + jt.cta, 1) == jt.n - 1;
+                    if (last) p.arrived[jt.cta] = 0;
+                    last_part = last;
+                }
+                __syncthreads();
+                if (last_part) {
+                    __threadfence();
+                    join_parts<DP>(p, jt, use.at, use.q, min(rows - row0, TR));
+                }
+            }
         }
         if (!use.next(p)) break;
         __syncthreads();
     }
     cp_wait<0>();
-}
-
-// Joins the parts of an item that spans CTAs: block (j, r) takes row r of the item whose first cut is
-// boundary j + 1.  A thread owns four neighbouring columns of every GROUPS-th part; the maximum comes first, so the parts'
-// loads are independent, and the groups' sums are added in a fixed order.
-template <int DP>
-__global__ void __launch_bounds__(128) k_attn_join_few(const __grid_constant__ AttnParams p) {
-    constexpr int COLS = DP / 4, GROUPS = 128 / COLS;
-    __shared__ float red[4];
-    __shared__ float4 sum[GROUPS][COLS];
-    __shared__ float lsum[GROUPS];
-    grid_dep_trigger_small();
-    grid_dep_wait();
-    Joint jt;
-    if (!find_joint<S>(p, (int)blockIdx.x + 1, jt)) return;
-    const Req q = load_req(p, jt.at.r);
-    const int r = (int)blockIdx.y, row = jt.at.t * TR + r;
-    if (row >= q.nq * (int)p.gd.d) return;
-    float mm = -INFINITY;
-    for (int i = threadIdx.x; i < jt.n; i += 128) mm = fmaxf(mm, p.part_ml[(jt.slot(i) * TR + r) * 2]);
-    for (int x = 16; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = mm;
-    __syncthreads();
-    mm = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float ref = mm == -INFINITY ? 0.0f : mm;
-    const int g = threadIdx.x / COLS, col = threadIdx.x % COLS;
-    float ll = 0.0f;
-    float4 o = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-    for (int i = g; i < jt.n; i += GROUPS) {
-        const size_t at = jt.slot(i) * TR + r;
-        const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + at * 2);
-        const float4 v = *reinterpret_cast<const float4 *>(p.part_o + at * DP + col * 4);
-        const float w = ex2(ml.x - ref);
-        ll += w * ml.y;
-        o.x += w * v.x;
-        o.y += w * v.y;
-        o.z += w * v.z;
-        o.w += w * v.w;
-    }
-    sum[g][col] = o;
-    if (col == 0) lsum[g] = ll;
-    __syncthreads();
-    if (g) return;
-    for (int i = 1; i < GROUPS; ++i) {
-        const float4 v = sum[i][col];
-        ll += lsum[i];
-        o.x += v.x;
-        o.y += v.y;
-        o.z += v.z;
-        o.w += v.w;
-    }
-    const bool some = ll > 0.0f || ll != ll;
-    const float inv = some ? 1.0f / ll : 0.0f;
-    const uint32_t tok = p.gd.div((uint32_t)row);
-    const uint32_t head = jt.at.h * p.gd.d + (row - tok * p.gd.d);
-    if (col * 4 < (int)p.head_dim) {
-        const uint64_t e = (uint64_t)(q.q0 + tok) * p.out_stride + (uint64_t)head * p.head_dim + col * 4;
-        if (p.io_type == T_F32)
-            *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + e) =
-                make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-        else
-            *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + e) =
-                make_uint2(pack2(p.io_type, o.x * inv, o.y * inv), pack2(p.io_type, o.z * inv, o.w * inv));
-    }
-    if (p.lse && col == 0)
-        p.lse[(uint64_t)(q.q0 + tok) * (p.n_kv * p.gd.d) + head] = some ? (mm + log2f(ll)) * LN2 : -INFINITY;
 }
 
 template <int TYPE, int DP, int TERMS>
@@ -496,9 +487,7 @@ int launch(AttnParams p, cudaStream_t s) {
     }
     const uint32_t grid = SMS * F::CTAS;
     p.part_ml = p.part_o + (size_t)grid * 2 * TR * DP;
-    cudaError_t e = launch_pdl(k_attn_few<TYPE, DP, TERMS>, dim3(grid), dim3(WARPS * 32), F::SMEM, s, p);
-    if (e == cudaSuccess) e = launch_pdl(k_attn_join_few<DP>, dim3(grid - 1, TR), dim3(128), 0, s, p);
-    return (int)e;
+    return (int)launch_pdl(k_attn_few<TYPE, DP, TERMS>, dim3(grid), dim3(WARPS * 32), F::SMEM, s, p);
 }
 template <int TYPE, int DP>
 int launch_terms(const AttnParams &p, cudaStream_t s) {

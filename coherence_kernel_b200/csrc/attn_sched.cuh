@@ -8,7 +8,9 @@
 // [c U / C, (c + 1) U / C): the split depends on the lengths alone, so ragged batches, one long
 // request and many short ones all fill the GPU evenly and results do not depend on timing.  An
 // item that spans CTAs leaves one partial result per CTA (running maximum, sum, unnormalised
-// output), which a second kernel joins in CTA order.
+// output), joined in CTA order: in the few-row form by the CTA that brings the last part, whoever it is (one
+// launch less: 2 us of a small call's host time), in the chunk form, whose parts are 256 rows, by a second kernel that
+// spreads them over the GPU (17 ragged requests 55 us, in the last CTA 69).
 //
 // The lengths are device data: every CTA sums the units of all requests itself (a few loads per
 // thread) instead of waiting for a planning kernel.
@@ -196,8 +198,10 @@ struct Sched {
         Req q;
         Geo g;
         int nt, left, c0, c1;
+        long long first;  // the item's first unit
         // false if the CTA has no unit with keys
-        CK_DEV bool set(const AttnParams &p, const Shared &sh, int n) {
+        CK_DEV bool set(const AttnParams &p, const Shared &sh, int n, long long u0 = 0) {
+            first = u0 - sh.pos.c;
             at = sh.pos;
             g = sh.geo;
             q = sh.req;
@@ -211,6 +215,7 @@ struct Sched {
         // the next item; false at the end of the CTA's range
         CK_DEV bool next(const AttnParams &p) {
             left -= g.nch + EXTRA - c0;
+            first += g.nch + EXTRA;
             if (left <= 0) return false;
             if (++at.h >= (int)p.n_kv) {
                 at.h = 0;
@@ -230,6 +235,22 @@ struct Sched {
         }
     };
 
+    // The parts of an item that spans CTAs: those of CTAs cta .. cta + n - 1, in each CTA's slot 0 except, where the
+    // item is not the first with keys in the first CTA's range, slot 1 there.
+    struct Joint {
+        int cta, n, slot0;
+        CK_DEV size_t slot(int i) const { return (size_t)(cta + i) * 2 + (i == 0 ? slot0 : 0); }
+    };
+    static CK_DEV Joint joint(const Items &it, long long U, int C) {
+        // the CTA of unit u is the largest c with U c / C <= u, that is c <= (C (u + 1) - 1) / U
+        const long long a = it.first, b = a + it.g.nch;
+        Joint j;
+        j.cta = (int)((C * (a + 1) - 1) / U);
+        j.n = (int)((C * b - 1) / U) - j.cta + 1;
+        j.slot0 = start(U, C, j.cta) >= a - EXTRA ? 0 : 1;  // a start behind the last item's keys is as good as a
+        return j;
+    }
+
     // What the joining kernel needs of each CTA's start, left in the workspace by the CTA.
     static CK_DEV void leave_cut(const AttnParams &p, long long U, int C, const Pos &at, const Geo &g) {
         if (threadIdx.x == 0) {
@@ -246,13 +267,13 @@ struct Sched {
 // An item that spans CTAs, seen from boundary j (the start of CTA j's units): found at its first cut only.
 // Its parts are those of CTAs first .. first + n - 1, in each CTA's slot 0 except, where the item is not the first
 // with keys in the first CTA's range, slot 1 there.
-struct Joint {
+struct Cut {
     Pos at;
     int first, n, slot0;
     CK_DEV size_t slot(int i) const { return (size_t)(first + i) * 2 + (i == 0 ? slot0 : 0); }
 };
 template <class S>
-CK_DEV bool find_joint(const AttnParams &p, int j, Joint &o) {
+CK_DEV bool find_joint(const AttnParams &p, int j, Cut &o) {
     const long long U = p.cuts->units;
     const int C = p.cuts->ctas;
     if (j >= C) return false;

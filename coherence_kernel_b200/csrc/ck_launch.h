@@ -200,7 +200,7 @@ int launch_kv_append(const KvAppendParams &p, int in_type, cudaStream_t s);
 
 // attention over the paged cache (attn_paged.cu, attn_chunk.cu)
 constexpr int ATTN_MAX_CTAS = 148 * 3;
-struct AttnCuts {  // where each CTA's units begin, for the kernel that joins partial results
+struct AttnCuts {  // where each CTA's units begin, for the kernel that joins the chunk form's parts
     long long units;
     int ctas, pad;
     int4 at[ATTN_MAX_CTAS];      // request, tile, head, key chunk
@@ -212,7 +212,8 @@ struct AttnParams {
     float *lse;
     const int32_t *table, *kv_len, *q_start;
     float *part_o, *part_ml;  // partial results of work items that span CTAs
-    AttnCuts *cuts;
+    AttnCuts *cuts;           // chunk form
+    int *arrived;             // few-row form: parts finished, by the item's first CTA; zero between calls
     int *err;                 // device error word (bounded waits)
     uint64_t q_stride, out_stride, table_stride, block_stride, token_stride, head_stride;
     uint32_t nreq, ntok, n_kv, head_dim, max_blocks, n_blocks;

@@ -141,7 +141,7 @@ class PagedAttention:
         self.ws_bytes = _lib.load().ck_paged_attention_workspace_bytes(n_heads, n_kv_heads, head_dim)
         if self.ws_bytes == 0:
             raise ValueError(f"unsupported heads: {n_heads} over {n_kv_heads} of {head_dim}")
-        self.ws = torch.empty(self.ws_bytes, dtype=torch.uint8, device=device)
+        self.ws = torch.zeros(self.ws_bytes, dtype=torch.uint8, device=device)
 
     def __call__(self, q, k_cache, v_cache, table, kv_len, q_start, scale: float | None = None, causal: bool = True,
                  window: int = 0, out=None, lse=None, return_lse: bool = False):
@@ -160,7 +160,7 @@ class PagedAttention:
         shape = (ntok, heads, dim)
         qs = _rows3(q, "q", shape, (k_cache.dtype, torch.float32), dev)
         if out is None:
-            out = torch.empty(shape, dtype=q.dtype, device=dev)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
             os_ = heads * dim
         else:
             os_ = _rows3(out, "out", shape, (q.dtype,), dev)

@@ -18,8 +18,12 @@ Q8_0_BLOCK_BYTES, Q4K_BLOCK_BYTES = 34, 144
 TYPE_NUMBERS = {torch.float32: 0, torch.float16: 1, "q8_0": 8, torch.bfloat16: 30}
 
 
+_get_device, _get_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def _stream():
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    # the current stream's handle without a Stream object, whose making shows in a small call's time
+    return ctypes.c_void_p(_get_stream(torch.cuda.current_device()))
 
 
 def _ptr(t):
@@ -196,7 +200,6 @@ _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 
 _FN = {}
-_get_device, _get_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 def _call(name, device, *args):
@@ -263,7 +266,7 @@ def rmsnorm_add(x, residual, gain, eps, out_dtype=None, out=None, residual_out=N
         os_ = 0
     else:
         if out is None:
-            out = torch.empty(shape, dtype=out_dtype, device=dev)
+            out = torch.empty_like(x, dtype=out_dtype, memory_format=torch.contiguous_format)
             os_ = hidden
         elif out.dtype != out_dtype:
             raise ValueError(f"out has dtype {out.dtype}, expected {out_dtype}")

@@ -406,8 +406,9 @@ int ck_kv_append(const ck_kv_config *cfg, int in_type, const void *k_dev, uint64
  * io_type (q and out): the cache's type, with P rounded to it once before the second product, or CK_F32, which
  * keeps fp32 accuracy.  q_stride, out_stride: elements between rows, multiples of 8.  n_heads is a multiple
  * of n_kv_heads, scale finite and > 0; ntok * n_heads < 2^30, max_blocks * block_tokens < 2^30.  ntok bounds the rows:
- * q_start[nreq] <= ntok.  workspace: ck_paged_attention_workspace_bytes (the same for every batch size); calls that overlap in
- * time need one each. */
+ * q_start[nreq] <= ntok.  workspace: ck_paged_attention_workspace_bytes (the same for every batch size), all zeros
+ * before the first call with it and after a CK_ETIMEOUT (it counts the parts of work that spans CTAs, and every call
+ * leaves the counts at zero); calls that overlap in time need one each. */
 size_t ck_paged_attention_workspace_bytes(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim);
 int ck_paged_attention(const ck_kv_config *cfg, uint32_t n_heads, int io_type, const void *q_dev, uint64_t q_stride,
                        const void *k_cache_dev, const void *v_cache_dev, const int32_t *table_dev, uint64_t table_stride,
@@ -427,7 +428,7 @@ int ck_paged_attention_status(const void *workspace_dev, void *stream);
  * [ntok, hidden], k and v fp32 [ntok, n_kv_heads * head_dim] are outputs.  The rows are the plan's: a batch
  * mixes decodes and chunks freely within max_tokens.  The struct and *cache are read during the call only;
  * a capture records the addresses in them, so that a plan that advances the same buffers before each
- * ck_decode_step_replay makes it the next step.  workspace: ck_paged_attention_workspace_bytes. */
+ * ck_decode_step_replay makes it the next step.  workspace: ck_paged_attention_workspace_bytes, zeroed first. */
 typedef struct {
     const ck_kv_config *cache;
     void *k_cache_dev, *v_cache_dev;
