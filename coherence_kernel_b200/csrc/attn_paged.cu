@@ -110,7 +110,7 @@ CK_DEV void join_parts(const AttnParams &p, const S::Joint &jt, const Pos &at, c
         const int r = i / COLS, col = i % COLS * 4;
         float m = -INFINITY, l = 0.0f;
         float4 o = make_float4(0, 0, 0, 0);
-#pragma unroll 8
+#pragma unroll 16
         for (int k = 0; k < jt.n; ++k) {
             const size_t s = jt.slot(k) * TR + r;
             const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p.part_ml + s * 2));

@@ -64,6 +64,7 @@ template <int TR, int KC, bool CHUNK>
 struct Sched {
     static constexpr int ALIGN = CHUNK ? 64 : 16;
     static constexpr int EXTRA = CHUNK ? 3 : 2;
+    static constexpr int PARTS = 128;
     static CK_DEV int tiles(const AttnParams &p, const Req &q) {
         const int rows = q.nq * (int)p.gd.d;
         if (CHUNK ? rows < (int)p.row_split : rows >= (int)p.row_split) return 0;
@@ -96,26 +97,33 @@ struct Sched {
 
     struct Shared {
         long long warp_sum[32];
+        int warp_items[32];
         long long before;
         Pos pos;
         Geo geo;
         Req req;
     };
-    // exclusive prefix of v over the CTA; `all` receives the sum
-    static CK_DEV long long scan(long long v, Shared &sh, long long &all) {
+    // exclusive prefix of v over the CTA; `all` receives the sum, `items` that of the threads' items
+    static CK_DEV long long scan(long long v, Shared &sh, long long &all, int &items) {
         const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
         long long s = v;
         for (int o = 1; o < 32; o <<= 1) {
             const long long u = __shfl_up_sync(0xffffffffu, s, o);
             if (lane >= o) s += u;
         }
-        if (lane == 31) sh.warp_sum[w] = s;
+        items = (int)__reduce_add_sync(0xffffffffu, (unsigned)items);
+        if (lane == 31) {
+            sh.warp_sum[w] = s;
+            sh.warp_items[w] = items;
+        }
         __syncthreads();
         long long before = 0;
         all = 0;
+        items = 0;
         for (int i = 0; i < nw; ++i) {
             if (i < w) before += sh.warp_sum[i];
             all += sh.warp_sum[i];
+            items = min(items + sh.warp_items[i], 1 << 20);
         }
         __syncthreads();
         return before + s - v;
@@ -125,22 +133,29 @@ struct Sched {
         return U < 1 << 22 ? (long long)((uint32_t)U * (uint32_t)c / (uint32_t)C) : U * c / C;
     }
 
-    // Called by the whole CTA.  Finds the total U, the CTAs that take part C = min(grid, U), and the
-    // position of unit start(cta); returns false when cta takes no part.
+    // Called by the whole CTA.  Finds the total U, the CTAs that take part C -- at most one a unit, and PARTS an item
+    // on average: joining a part costs about a tenth of a unit -- and the position of unit start(cta); returns false
+    // when cta takes no part.
     static CK_DEV bool find(const AttnParams &p, Shared &sh, int grid, int cta, long long &U, int &C, Pos &pos, Geo &geo) {
         const int n = (int)p.nreq, bd = (int)blockDim.x;
         Req q;
         long long mine = units(p, threadIdx.x, q), sum = mine;
-        for (int b = bd; b < n; b += bd) sum += units(p, b + (int)threadIdx.x);
-        long long ex = scan(sum, sh, U);
+        int items = (int)min((long long)tiles(p, q) * p.n_kv, 1ll << 16);
+        for (int b = bd; b < n; b += bd) {
+            Req o;
+            sum += units(p, b + (int)threadIdx.x, o);
+            items = min(items + (int)min((long long)tiles(p, o) * p.n_kv, 1ll << 16), 1 << 16);
+        }
+        long long ex = scan(sum, sh, U, items);
         C = (int)(U < grid ? U : grid);
+        C = min(C, PARTS * items);
         if (cta >= C) return false;
         const long long u = start(U, C, cta);
         if (n > bd) {  // more requests than threads: once more, block by block
             long long base = 0, all = 0;
             for (int b = 0;; b += bd) {
                 mine = units(p, b + (int)threadIdx.x, q);
-                ex = base + scan(mine, sh, all);
+                ex = base + scan(mine, sh, all, items);
                 if (u >= ex && u < ex + mine) sh.pos.r = b + (int)threadIdx.x;
                 if (u < base + all) break;
                 base += all;
