@@ -6,9 +6,9 @@
 // in one pass over the keys with the running maximum and sum of each row.  The rows of a tile are 16
 // (token, grouped query head) pairs that share a K/V head, so each K and V row is read once for all
 // of them.  HBM bounds it: a decode step does 4 x rows flop per cache element.  One token over 131,072 (32 heads over 8,
-// f16): 93 us for both launches, 5.8 TB/s, 89% of the measured copy rate; 64 ragged decodes of up to 8192 tokens 193 us
+// f16): 92 us, 5.8 TB/s, 89% of the measured copy rate; 64 ragged decodes of up to 8192 tokens 193 us
 // (88%).  Short contexts are bound by latency: one token over 1000 with 56 heads in the f32 form 20 us, of which finding
-// the work 2, the first keys 2, three units 5, joining warps 2 and joining CTAs 5.
+// the work 2, the first keys 2, three units 5, joining warps and CTAs 4, the rest launch and skew.
 //
 // A CTA has four warps.  A unit is 64 keys; each warp takes 16 of them and has a ring of its own of
 // STAGES x (16 K rows + 16 V rows) in shared memory, filled by 16-byte asynchronous copies whose
@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
             }
         }
         {
-            // join the warps: common maximum, then the scaled sums warp by warp
+            // join the warps under their common maximum
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 l[k] += __shfl_xor_sync(0xffffffffu, l[k], 1);

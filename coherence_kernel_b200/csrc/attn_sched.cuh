@@ -1,16 +1,17 @@
 // attn_sched.cuh -- how the attention kernels share their work out over a fixed number of CTAs.
 //
 // An item is one tile of TR rows (rows = tokens x the query heads of one K/V head, token-major) of
-// one request and K/V head; a unit is KC consecutive keys of an item.  An item also counts for EXTRA units without
-// keys at its end: what its queries' load and its epilogue cost, so that a CTA of many short items gets no more
-// work than one of a long one (64 ragged decodes, 1 to 8192 tokens: the slowest CTA took twice the median's time).  Units are numbered request
-// by request, tile by tile, head by head, key chunk by key chunk, and CTA c of C takes units
-// [c U / C, (c + 1) U / C): the split depends on the lengths alone, so ragged batches, one long
-// request and many short ones all fill the GPU evenly and results do not depend on timing.  An
-// item that spans CTAs leaves one partial result per CTA (running maximum, sum, unnormalised
-// output), joined in CTA order: in the few-row form by the CTA that brings the last part, whoever it is (one
-// launch less: 2 us of a small call's host time), in the chunk form, whose parts are 256 rows, by a second kernel that
-// spreads them over the GPU (17 ragged requests 55 us, in the last CTA 69).
+// one request and K/V head; a unit is KC consecutive keys of an item.  An item also counts for EXTRA
+// units without keys at its end: what its queries' load and its epilogue cost, so that a CTA of many
+// short items gets no more work than one of a long one (64 ragged decodes, 1 to 8192 tokens: the
+// slowest CTA took twice the median's time).  Units are numbered request by request, tile by tile,
+// head by head, key chunk by key chunk, and CTA c of C takes units [c U / C, (c + 1) U / C): the split
+// depends on the lengths alone, so ragged batches, one long request and many short ones all fill the
+// GPU evenly and results do not depend on timing.  An item that spans CTAs leaves one partial result
+// per CTA (running maximum, sum, unnormalised output), joined in CTA order: in the few-row form by the
+// CTA that brings the last part, whoever it is (one launch less: 2 us of a small call's host time), in
+// the chunk form, whose parts are 256 rows, by a second kernel that spreads them over the GPU (17
+// ragged requests 55 us; in the last CTA 69).
 //
 // The lengths are device data: every CTA sums the units of all requests itself (a few loads per
 // thread) instead of waiting for a planning kernel.
