@@ -64,35 +64,38 @@ def _ints(t, name, n, device):
 
 def _rows3(t, name, shape, kinds, device):
     """A tensor [n, heads, dim] of this shape with contiguous rows; returns the row stride."""
-    st = t.stride()
     if t.shape != shape or t.dtype not in kinds or t.device != device:
         raise ValueError(f"{name} must be {list(shape)} on {device}, of {' or '.join(map(str, kinds))}")
     n, h, d = shape
-    if (st[2] != 1 and d > 1) or (st[1] != d and h > 1) or (n > 1 and st[0] < h * d):
+    row, head, one = t.stride()
+    if (one != 1 and d > 1) or (head != d and h > 1) or (row < h * d and n > 1):
         raise ValueError(f"{name}'s rows must be contiguous")
-    return st[0] if n > 1 else h * d
+    return row if n > 1 else h * d
 
 
 def _table(t, device):
-    st = t.stride()
+    row, col = t.stride()
     n, w = t.shape
-    if t.dtype is not _I32 or t.device != device or (w > 1 and st[1] != 1) or (n > 1 and st[0] < w):
+    if t.dtype is not _I32 or t.device != device or (col != 1 and w > 1) or (row < w and n > 1):
         raise ValueError(f"table must be int32 [nreq, max_blocks] on {device} with contiguous rows")
-    return st[0] if n > 1 else w
+    return row if n > 1 else w
 
 
 def plan(table, length, new_tokens, free_blocks, free_count, block_tokens: int, ntok: int, out: Plan | None = None) -> Plan:
     """Block tables and slot maps of one step (ck_kv_plan): table int32 [nreq, max_blocks] and
     free_blocks int32 [n_blocks] are updated in place; length and free_count are read, and the new
     ones are in the returned plan (whose tensors may be these)."""
-    dev = table.device
-    if not table.is_cuda or table.dim() != 2:
+    dev, shape = table.device, table.shape
+    if dev.type != "cuda" or len(shape) != 2:
         raise ValueError("table must be a CUDA tensor [nreq, max_blocks]")
-    nreq, max_blocks = table.shape
+    nreq, max_blocks = shape
     stride = _table(table, dev)
-    o = out if out is not None else plan_buffers(nreq, ntok, dev)
-    if o.length.numel() < nreq or o.slots.numel() < ntok or o.length.device != dev:
-        raise ValueError(f"out holds less than {nreq} requests and {ntok} rows, or is not on {dev}")
+    if out is None:
+        o = plan_buffers(nreq, ntok, dev)
+    else:
+        o = out
+        if o.length.numel() < nreq or o.slots.numel() < ntok or o.length.device != dev:
+            raise ValueError(f"out holds less than {nreq} requests and {ntok} rows, or is not on {dev}")
     _call("ck_kv_plan", dev, _ints(length, "length", nreq, dev), _ints(new_tokens, "new_tokens", nreq, dev), nreq,
           table.data_ptr(), stride, max_blocks, _ints(free_blocks, "free_blocks", 1, dev),
           _ints(free_count, "free_count", 1, dev), free_blocks.numel(), block_tokens, ntok, o.length.data_ptr(),
@@ -104,14 +107,14 @@ def plan(table, length, new_tokens, free_blocks, free_count, block_tokens: int, 
 def _config(k_cache, v_cache):
     """ck_kv_config of cache tensors [n_blocks, block_tokens, n_kv_heads, head_dim] (any strides with
     contiguous heads, so a [n_blocks, n_kv_heads, block_tokens, head_dim] cache is passed permuted)."""
-    kt, st = k_cache.dtype, k_cache.stride()
-    if len(st) != 4 or k_cache.shape != v_cache.shape or kt != v_cache.dtype or st != v_cache.stride() or st[3] != 1:
+    kt, st, shape, dev = k_cache.dtype, k_cache.stride(), k_cache.shape, k_cache.device
+    if len(st) != 4 or shape != v_cache.shape or kt is not v_cache.dtype or st != v_cache.stride() or st[3] != 1:
         raise ValueError("k_cache and v_cache must be 4-dimensional, of one shape, type and strides, heads contiguous")
     if kt is not torch.bfloat16 and kt is not torch.float16:
         raise ValueError(f"the cache has dtype {kt}, expected bfloat16 or float16")
-    if not k_cache.is_cuda or v_cache.device != k_cache.device:
+    if dev.type != "cuda" or v_cache.device != dev:
         raise ValueError("the cache must be CUDA tensors on one device")
-    nb, bt, h, d = k_cache.shape
+    nb, bt, h, d = shape
     return _lib.KvConfig(h, d, bt, nb, TYPE_NUMBERS[kt], 0, st[0], st[1], st[2])
 
 

@@ -206,8 +206,9 @@ def _call(name, device, *args):
     """The C call on the device's current stream, appended to the arguments; raises on an error code.  A
     device guard only where the tensors lie on another device than the current one: its cost, like
     that of a Stream object, shows in a small call's time."""
-    fn = _FN.get(name)
-    if fn is None:
+    try:
+        fn = _FN[name]
+    except KeyError:
         fn = _FN[name] = getattr(_lib.load(), name)
     i = device.index
     if i == _get_device():
