@@ -17,12 +17,14 @@
 // fifth-generation instructions start at 64), with fp32 accumulation; P goes from the first product's
 // registers to the second's operands.
 //
-// With f32 queries and outputs the operands keep fp32's accuracy: Q and P are split into TERMS terms
-// of the cache's type, each the rounding of the remainder (bf16: three of 8 bits; f16: two of 11, Q's rows
-// scaled to [1, 2) by a power of two first), and every product with a K or V element is exact in the
-// accumulator.  (A remainder may be zero or negative, so infinities of V are kept out of every such product and
-// added afterwards.)  With 2-byte queries P is rounded once to the cache's type, an error of half an ulp of each
-// weight, below the output's own rounding.
+// With f32 queries and outputs the operands keep fp32's accuracy and range, and every product with a K or V element
+// is exact in the accumulator.  bf16 caches: Q and P are split into three bf16 terms of 8 bits, each the rounding of
+// the remainder.  f16 caches: into two tf32 terms of 11 bits, an f16 element being a tf32 value (64 ragged decodes of
+// up to 8192 tokens 319 us; with three bf16 terms, each element the sum of two bf16 values, 377).  f16 terms would
+// take half the products (246 us), but have no room for small weights and query elements: those under 2^-14 lose
+// bits, those under 2^-25 are lost.  A remainder may be zero or negative, so infinities of V are kept out of every
+// such product and added afterwards.  With 2-byte queries P is rounded once to the cache's type, an error of half an
+// ulp of each weight, below the output's own rounding.
 #include "attn_sched.cuh"
 
 #include <type_traits>
@@ -34,6 +36,7 @@ namespace {
 constexpr int TR = 16, KC = 64, WARPS = 4, WK = KC / WARPS;  // rows, keys per unit, warps, keys per warp
 using S = Sched<TR, KC, false>;
 
+// TERMS: 1 for 2-byte queries; for f32 ones three (bf16) or two (tf32, f16 caches)
 template <int DP, int TERMS>
 struct Few {
     static constexpr int ROW = DP * 2;  // bytes of a K or V row in shared memory
@@ -42,7 +45,7 @@ struct Few {
     static constexpr int RING = WARPS * STAGES * STAGE;
     // the query tile (all terms), and after the last key two 16 x DP fp32 sums over two warps each
     static constexpr int QO = DP * 8 * TR;
-    static_assert(TERMS * ROW <= DP * 8, "the query tile's terms");
+    static_assert((TERMS == 2 ? 2 * DP * 4 : TERMS * ROW) <= DP * 8, "the query tile's terms");
     static constexpr int SMEM = RING + QO;
     static constexpr int CTAS = DP <= 64 ? 3 : DP <= 128 ? 2 : 1;  // per SM
 };
@@ -78,19 +81,35 @@ CK_DEV void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// the pair (lo, hi) rounded to the type, and the remainders left in lo, hi
-template <int TYPE>
+// the pair (lo, hi) rounded to bf16, and the remainders left in lo, hi
 CK_DEV uint32_t split2(float &lo, float &hi) {
-    const uint32_t w = pack2(TYPE, lo, hi);
-    if constexpr (TYPE == T_BF16) {
-        lo -= __uint_as_float(w << 16);
-        hi -= __uint_as_float(w & 0xFFFF0000u);
-    } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
-        lo -= f.x;
-        hi -= f.y;
-    }
+    const uint32_t w = pack_bf16x2(lo, hi);
+    lo -= __uint_as_float(w << 16);
+    hi -= __uint_as_float(w & 0xFFFF0000u);
     return w;
+}
+// v rounded to tf32, and the remainder left in v
+CK_DEV float split_tf32(float &v) {
+    uint32_t w;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(w) : "f"(v));
+    const float t = __uint_as_float(w & 0xFFFFE000u);
+    v -= t;
+    return t;
+}
+// 16 x 8 by 8 x 8 in tf32; b: two f16 elements of a column.  A fragment's k runs over a thread's pairs in the order
+// first elements, second elements, in a and b alike.
+CK_DEV void mma_tf32(float (&c)[4], const float (&a)[4], uint32_t b) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&b));
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(__float_as_uint(a[0])), "r"(__float_as_uint(a[1])), "r"(__float_as_uint(a[2])),
+                   "r"(__float_as_uint(a[3])), "r"(__float_as_uint(f.x)), "r"(__float_as_uint(f.y)));
+}
+// byte offset of element e (even) of row r in a query tile of tf32 terms: 16-byte pieces, swizzled so that the eight bytes
+// of four rows by four neighbouring threads fall into different banks
+template <int DP>
+CK_DEV uint32_t tf32_at(int term, int r, int e) {
+    return (uint32_t)((term * TR + r) * DP * 4 + ((((e >> 2) ^ ((r & 3) << 1)) << 4) | (e & 3) * 4));
 }
 // a pair of V elements with its infinities and NaNs replaced by zero
 template <int TYPE>
@@ -146,10 +165,12 @@ CK_DEV void join_parts(const AttnParams &p, const S::Joint &jt, const Pos &at, c
 template <int TYPE, int DP, int TERMS>
 __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(const __grid_constant__ AttnParams p) {
     using F = Few<DP, TERMS>;
+    constexpr bool TF = TERMS == 2;
+    static_assert(TERMS == 1 || TF == (TYPE == T_F16), "terms of the cache's type");
     constexpr int ROW = F::ROW, NS = F::STAGES, PIECES = DP / 8, COPIES = WK * PIECES / 32;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ typename S::Shared sh;
-    __shared__ float row_scale[TR], wm[WARPS][TR], wl[WARPS][TR];
+    __shared__ float wm[WARPS][TR], wl[WARPS][TR];
     __shared__ int last_part;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t ring = smem_u32(smem) + warp * NS * F::STAGE, qs = smem_u32(smem) + F::RING;
@@ -234,39 +255,31 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
                 }
             } else {
                 float v[DP / 64][8];
-                float mx = 0.0f;
 #pragma unroll
                 for (int k = 0; k < DP / 64; ++k) {
                     const int c = part + 8 * k;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[k][e] = 0.0f;
                     if (live && c * 8 < (int)p.head_dim) raw8_to_float(load_raw8(p.q, at + c * 8, T_F32), T_F32, v[k]);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(v[k][e]));
                 }
-                float back = 1.0f;
-                if constexpr (TYPE == T_F16) {
-                    // scale the row's largest |q| into [1, 2): f16's range then holds both terms
-                    for (int x = 1; x < 8; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-                    const int ex = min(max((int)(__float_as_uint(mx) >> 23) - 127, -100), 100);
-                    const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
-                    back = __uint_as_float((uint32_t)(127 + ex) << 23);
-#pragma unroll
-                    for (int k = 0; k < DP / 64; ++k)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[k][e] *= down;
-                }
-                if (part == 0) row_scale[r] = back;
 #pragma unroll
                 for (int term = 0; term < TERMS; ++term)
 #pragma unroll
                     for (int k = 0; k < DP / 64; ++k) {
                         const int c = part + 8 * k;
+                        if constexpr (TF) {
+#pragma unroll
+                            for (int e = 0; e < 8; e += 4)
+                                *reinterpret_cast<float4 *>(smem + F::RING + tf32_at<DP>(term, r, c * 8 + e)) =
+                                    make_float4(split_tf32(v[k][e]), split_tf32(v[k][e + 1]), split_tf32(v[k][e + 2]),
+                                                split_tf32(v[k][e + 3]));
+                            continue;
+                        }
                         uint4 w;
-                        w.x = split2<TYPE>(v[k][0], v[k][1]);
-                        w.y = split2<TYPE>(v[k][2], v[k][3]);
-                        w.z = split2<TYPE>(v[k][4], v[k][5]);
-                        w.w = split2<TYPE>(v[k][6], v[k][7]);
+                        w.x = split2(v[k][0], v[k][1]);
+                        w.y = split2(v[k][2], v[k][3]);
+                        w.z = split2(v[k][4], v[k][5]);
+                        w.w = split2(v[k][6], v[k][7]);
                         *reinterpret_cast<uint4 *>(smem + F::RING + term * TR * ROW + r * ROW + ((c ^ (r & 7)) << 4)) = w;
                     }
             }
@@ -300,6 +313,18 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
                 }
 #pragma unroll
                 for (int term = 0; term < TERMS; ++term) {
+                    if constexpr (TF) {
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const int r = lane >> 2, e = ks * 16 + x * 8 + (lane & 3) * 2;
+                            const float2 u = *reinterpret_cast<const float2 *>(smem + F::RING + tf32_at<DP>(term, r, e));
+                            const float2 w = *reinterpret_cast<const float2 *>(smem + F::RING + tf32_at<DP>(term, r + 8, e));
+                            const float a[4] = {u.x, w.x, u.y, w.y};
+                            mma_tf32(sk[0], a, b[x]);
+                            mma_tf32(sk[1], a, b[2 + x]);
+                        }
+                        continue;
+                    }
                     uint32_t a[4];
                     const int r = lane & 15, c = ks * 2 + (lane >> 4);
                     ldsm4(qs + term * TR * ROW + r * ROW + ((c ^ (r & 7)) << 4), a);
@@ -314,13 +339,12 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
             const bool partial = j0 < all_lo || j0 + WK > all_hi;  // some row does not see some key
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const float sc = TERMS > 1 && TYPE == T_F16 ? p.scale_log2 * row_scale[(lane >> 2) + 8 * k] : p.scale_log2;
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         float &x = s[t][2 * k + e];
-                        x *= sc;
+                        x *= p.scale_log2;
                         if (partial) {
                             const int j = j0 + t * 8 + (lane & 3) * 2 + e;
                             if (j < row_lo[k] || j >= row_hi[k]) x = -INFINITY;
@@ -350,14 +374,37 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
                         l[k] += x;
                     }
             }
+            if constexpr (TF) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {  // eight keys, by the 32 dims of a step
+                    float a[TERMS][4];
+#pragma unroll
+                    for (int term = 0; term < TERMS; ++term)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) a[term][x] = split_tf32(s[t][(x & 1) * 2 + (x >> 1)]);
+#pragma unroll
+                    for (int dt = 0; dt < DP / 32; ++dt) {
+                        uint32_t b[4];
+                        const int key = t * 8 + (lane & 7), c = dt * 4 + (lane >> 3);
+                        ldsm4t(vb + key * ROW + ((c ^ (key & 7)) << 4), b);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            b[x] = finite2<TYPE>(b[x], bad);
+#pragma unroll
+                            for (int term = 0; term < TERMS; ++term) mma_tf32(o[4 * dt + x], a[term], b[x]);
+                        }
+                    }
+                }
+                continue;
+            }
             uint32_t a[TERMS][4];
 #pragma unroll
-            for (int term = 0; term < TERMS; ++term) {
-                a[term][0] = split2<TYPE>(s[0][0], s[0][1]);
-                a[term][1] = split2<TYPE>(s[0][2], s[0][3]);
-                a[term][2] = split2<TYPE>(s[1][0], s[1][1]);
-                a[term][3] = split2<TYPE>(s[1][2], s[1][3]);
-            }
+            for (int term = 0; term < TERMS; ++term)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    float &lo = s[x >> 1][(x & 1) * 2], &hi = s[x >> 1][(x & 1) * 2 + 1];
+                    a[term][x] = TERMS > 1 ? split2(lo, hi) : pack2(TYPE, lo, hi);
+                }
 #pragma unroll
             for (int dt = 0; dt < DP / 16; ++dt) {
                 uint32_t b[4];
