@@ -24,7 +24,9 @@
 // take half the products (246 us), but have no room for small weights and query elements: those under 2^-14 lose
 // bits, those under 2^-25 are lost.  A remainder may be zero or negative, so infinities of V are kept out of every
 // such product and added afterwards.  With 2-byte queries P is rounded once to the cache's type, an error of half an
-// ulp of each weight, below the output's own rounding.
+// ulp of each weight, below the output's own rounding.  f16 weights are taken times LIFT = 2^15 (they stay below
+// 65504), so that only those under 2^-29 of their row's largest fall among f16's subnormals, where a weight is off by
+// at most 2^-40 of the largest.
 #include "attn_sched.cuh"
 
 #include <type_traits>
@@ -166,6 +168,7 @@ template <int TYPE, int DP, int TERMS>
 __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(const __grid_constant__ AttnParams p) {
     using F = Few<DP, TERMS>;
     constexpr bool TF = TERMS == 2;
+    constexpr float LIFT = TERMS == 1 && TYPE == T_F16 ? 32768.0f : 1.0f;
     static_assert(TERMS == 1 || TF == (TYPE == T_F16), "terms of the cache's type");
     constexpr int ROW = F::ROW, NS = F::STAGES, PIECES = DP / 8, COPIES = WK * PIECES / 32;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -403,7 +406,7 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                     float &lo = s[x >> 1][(x & 1) * 2], &hi = s[x >> 1][(x & 1) * 2 + 1];
-                    a[term][x] = TERMS > 1 ? split2(lo, hi) : pack2(TYPE, lo, hi);
+                    a[term][x] = TERMS > 1 ? split2(lo, hi) : pack2(TYPE, lo * LIFT, hi * LIFT);
                 }
 #pragma unroll
             for (int dt = 0; dt < DP / 16; ++dt) {
@@ -439,7 +442,7 @@ __global__ void __launch_bounds__(WARPS * 32, Few<DP, TERMS>::CTAS) k_attn_few(c
                 const int r = (lane >> 2) + 8 * k;
                 float mm = wm[0][r];
                 for (int w = 1; w < WARPS; ++w) mm = fmaxf(mm, wm[w][r]);
-                f[k] = ex2(m[k] - (mm == -INFINITY ? 0.0f : mm));
+                f[k] = ex2(m[k] - (mm == -INFINITY ? 0.0f : mm)) * (1.0f / LIFT);
             }
             // warps 0 and 1 lay their sums down, 2 and 3 add theirs to them
 #pragma unroll

@@ -59,3 +59,12 @@ def test_f32_rows_keep_small_query_elements(cache, dim):
         q, k = q.clone(), k.clone()
         q[..., 3], k[..., 3] = big, 0.0
         check((q / 4 if big < 1e30 else q, k, v, table, kl, starts))
+
+
+@pytest.mark.parametrize("gap", GAPS)
+@pytest.mark.parametrize("cache", [BF16, F16])
+@pytest.mark.parametrize("jitter", [0.0, 0.5])
+def test_16_bit_rows_keep_small_weights(gap, cache, jitter):
+    lost = 2.0 ** -40 if cache == F16 else 0.0
+    check(sink_case(gap, jitter, [(1024, 1), (300, 3), (9, 2)], 2, 1, 64, 16, cache, cache), lost)
+    check(sink_case(gap, jitter, [(700, 1)], 3, 3, 128, 16, cache, cache), lost)
