@@ -20,7 +20,10 @@
 // O is rescaled only when a row's maximum has grown by more than 8 (in log2 units) since the maximum
 // its weights refer to: weights stay below 2^8, exactly representable scaling, and most units skip the
 // round trip of O through registers.  P is rounded once to the cache's type (half an ulp of each weight,
-// below the output's own rounding); scores, sums and O are fp32.
+// below the output's own rounding); scores, sums and O are fp32.  f16 weights are taken times 2^13 and rescaled at a
+// growth of 2, which keeps them below 65504: only those under 2^-27 of their row's largest fall among f16's
+// subnormals, where a weight is off by at most 2^-38 of the largest.  The maximum they refer to is rounded to a whole
+// number, so that neither the shift nor taking it back rounds anything (2048 new tokens of 8192: 249 us, as in bf16).
 //
 // Bounds per unit: the tensor core (4 x 128 x 128 x 128 multiply-adds, 2048 cycles), the exponentials (2 x 128 x 128 at 16
 // per cycle, 2048 cycles) and the tiles' way from L2 (64 KB at about 26 bytes per cycle, 2500 cycles) are close to
@@ -38,7 +41,6 @@ namespace {
 constexpr int TR = 256, KC = 128;
 using S = Sched<TR, KC, true>;
 constexpr int NTHREADS = 512;
-constexpr float GROW = 8.0f;  // log2 growth of a row's maximum that makes O rescale
 
 template <int DP>
 struct Chunk {
@@ -509,6 +511,9 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     } else {
         // -------------------------------------------------------------------------------- softmax
         reg_inc<184>();
+        // log2 growth of a row's maximum that makes O rescale, and the power of two that weights are raised by
+        constexpr float GROW = TYPE == T_F16 ? 2.0f : 8.0f, LIFT = TYPE == T_F16 ? 13.0f : 0.0f;
+        constexpr float DOWN = TYPE == T_F16 ? 0x1p-13f : 1.0f;
         const int t = wg, r = threadIdx.x & 127;  // tile of the item, row of the tile
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 lanes: lane number << 16
         const uint32_t s_at = tmem + s_col(t) + lanes, o_at = tmem + o_col(t) + lanes;
@@ -565,14 +570,15 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                                              __uint_as_float(s[2][31])),
                                         max3(mx[2], mx[3], __uint_as_float(s[3][31]))) *
                                   p.scale_log2;
+                const float whole_top = LIFT != 0.0f ? rintf(top) : top;
                 if (c == it.c0) {
-                    m = top;
+                    m = whole_top;
                 } else {
                     const bool grow = top > m + GROW || (m == -INFINITY && top > m);
                     if (__any_sync(0xffffffffu, grow)) {
                         // S_t of this unit completed, so PV_t of the last one has too: O is at rest until P_t is
                         // handed over
-                        const float mn = grow ? top : m;
+                        const float mn = grow ? whole_top : m;
                         const float al = grow ? ex2(m - mn) : 1.0f;
                         m = mn;
                         l *= al;
@@ -587,7 +593,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                         }
                     }
                 }
-                const float ref = m == -INFINITY ? 0.0f : m;
+                const float ref = (m == -INFINITY ? 0.0f : m) - LIFT;
                 const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), rf2 = make_float2(-ref, -ref);
                 float2 sum[2] = {make_float2(0, 0), make_float2(0, 0)};
 #pragma unroll
@@ -623,8 +629,9 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             const bool whole = it.whole();
             const int row = row0 + r;
             const bool live = row < rows;
+            l *= DOWN;
             const bool some = l > 0.0f || l != l;
-            const float inv = whole ? (some ? 1.0f / l : 0.0f) : 1.0f;
+            const float inv = whole ? (some ? DOWN / l : 0.0f) : DOWN;
             const uint32_t tok = p.gd.div((uint32_t)(live ? row : 0));
             const uint32_t head = it.at.h * p.gd.d + ((live ? row : 0) - tok * p.gd.d);
             const uint64_t oe = (uint64_t)(it.q.q0 + tok) * p.out_stride + (uint64_t)head * p.head_dim;

@@ -68,3 +68,12 @@ def test_16_bit_rows_keep_small_weights(gap, cache, jitter):
     lost = 2.0 ** -40 if cache == F16 else 0.0
     check(sink_case(gap, jitter, [(1024, 1), (300, 3), (9, 2)], 2, 1, 64, 16, cache, cache), lost)
     check(sink_case(gap, jitter, [(700, 1)], 3, 3, 128, 16, cache, cache), lost)
+
+
+@pytest.mark.parametrize("gap", GAPS)
+@pytest.mark.parametrize("cache", [BF16, F16])
+@pytest.mark.parametrize("dim,bt", [(64, 16), (128, 12)])
+def test_chunks_keep_small_weights(gap, cache, dim, bt):
+    lost = 2.0 ** -38 if cache == F16 else 0.0
+    check(sink_case(gap, 0.5, [(1100, 100), (90, 90)], 2, 1, dim, bt, cache, cache), lost)
+    check(sink_case(gap, 0.0, [(700, 70)], 2, 2, dim, bt, cache, cache), lost)
