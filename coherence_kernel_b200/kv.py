@@ -45,6 +45,16 @@ class Plan:
             if t.device != self.length.device:
                 raise ValueError("the plan's buffers must be on one device")
 
+    def cut(self, nreq: int, ntok: int) -> Plan:
+        """The plan of nreq requests and ntok rows in these buffers: itself, or views of their first elements."""
+        if (self.kv_len.numel() == nreq and self.slots.numel() == ntok and self.length.numel() == nreq
+                and self.q_start.numel() == nreq + 1 and self.positions.numel() == ntok):
+            return self
+        if self.length.numel() < nreq or self.slots.numel() < ntok:
+            raise ValueError(f"out holds less than {nreq} requests and {ntok} rows")
+        return Plan(self.length[:nreq], self.kv_len[:nreq], self.q_start[:nreq + 1], self.slots[:ntok],
+                    self.positions[:ntok], self.free_count)
+
 
 def plan_buffers(nreq: int, ntok: int, device) -> Plan:
     """Output buffers of `plan` for steps of nreq requests and ntok rows."""
@@ -84,7 +94,8 @@ def _table(t, device):
 def plan(table, length, new_tokens, free_blocks, free_count, block_tokens: int, ntok: int, out: Plan | None = None) -> Plan:
     """Block tables and slot maps of one step (ck_kv_plan): table int32 [nreq, max_blocks] and
     free_blocks int32 [n_blocks] are updated in place; length and free_count are read, and the new
-    ones are in the returned plan (whose tensors may be these)."""
+    ones are in the returned plan (whose tensors may be these).  out may be larger than the step: the
+    returned plan is then its first nreq requests and ntok rows."""
     dev, shape = table.device, table.shape
     if dev.type != "cuda" or len(shape) != 2:
         raise ValueError("table must be a CUDA tensor [nreq, max_blocks]")
@@ -93,9 +104,9 @@ def plan(table, length, new_tokens, free_blocks, free_count, block_tokens: int, 
     if out is None:
         o = plan_buffers(nreq, ntok, dev)
     else:
-        o = out
-        if o.length.numel() < nreq or o.slots.numel() < ntok or o.length.device != dev:
-            raise ValueError(f"out holds less than {nreq} requests and {ntok} rows, or is not on {dev}")
+        if out.length.device != dev:
+            raise ValueError(f"out is not on {dev}")
+        o = out.cut(nreq, ntok)
     _call("ck_kv_plan", dev, _ints(length, "length", nreq, dev), _ints(new_tokens, "new_tokens", nreq, dev), nreq,
           table.data_ptr(), stride, max_blocks, _ints(free_blocks, "free_blocks", 1, dev),
           _ints(free_count, "free_count", 1, dev), free_blocks.numel(), block_tokens, ntok, o.length.data_ptr(),
@@ -206,7 +217,8 @@ class PagedKV:
     def plan(self, new_tokens, ntok: int, out: Plan | None = None) -> Plan:
         """Advance the state by one step: request r gets new_tokens[r] rows (int32, on the device), or
         drops its last -new_tokens[r] tokens; ntok >= the step's rows.  Requests are rows 0 .. n - 1 of
-        the state, n = len(new_tokens)."""
+        the state, n = len(new_tokens).  The step's append and attention take the returned plan, which
+        holds n requests and ntok rows also where `out` has room for more."""
         n = new_tokens.numel()
         if n > self.max_requests or ntok > self.max_tokens:
             raise ValueError("more requests or rows than the cache was made for")

@@ -1,0 +1,43 @@
+"""Plans of a paged cache at their edges: buffers larger than the step, counts that saturate, padded batches."""
+import pytest
+import torch
+
+from coherence_kernel_b200 import kv
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def cache(**kw):
+    a = dict(n_blocks=16, block_tokens=4, n_heads=4, n_kv_heads=2, head_dim=64, max_requests=3, max_blocks=4, max_tokens=8)
+    return kv.PagedKV(**{**a, **kw})
+
+
+def test_larger_buffers_serve_a_smaller_step():
+    """A plan into buffers of an earlier, larger step holds this step's requests and rows only."""
+    g = torch.Generator().manual_seed(1)
+    q, k, v = (torch.randn(8, h, 64, generator=g).cuda() for h in (4, 2, 2))
+    got = []
+    for larger in (False, True):
+        c = cache()
+        buf = c.step_buffers(3, 8) if larger else None
+        p = c.plan(i32([2, 3, 1]), 8, out=buf)
+        c.append(k, v, p)
+        c.attend(q, p)
+        p = c.plan(i32([1, 1]), 2, out=buf)
+        assert [t.numel() for t in (p.length, p.kv_len, p.q_start, p.slots, p.positions)] == [2, 2, 3, 2, 2]
+        assert p.length.tolist() == [3, 4] and p.q_start.tolist() == [0, 1, 2]
+        with pytest.raises(ValueError):
+            c.append(k[:3], v[:3], p)  # the plan has two rows
+        c.append(k[6:], v[6:], p)
+        out = torch.full_like(q, 77.0)
+        c.attend(q, p, out=out)
+        assert (out[2:] == 77.0).all()  # no row of the third request, which is not in the step
+        got.append((out, c.k.clone(), c.v.clone(), c.length.clone()))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
