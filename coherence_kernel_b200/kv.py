@@ -26,13 +26,23 @@ from .ops import _FLOATS, TYPE_NUMBERS, _call, _dev, _ptr, _stream
 
 @dataclass
 class Plan:
-    """What ck_kv_plan wrote: one step's view of the cache.  Its buffers are checked once, here."""
+    """What ck_kv_plan wrote: one step's view of the cache.  Its buffers are checked when they are set."""
     length: torch.Tensor      # int32 [nreq] tokens held
     kv_len: torch.Tensor      # int32 [nreq] tokens the request's rows attend over (0: not served)
     q_start: torch.Tensor     # int32 [nreq + 1] first row of each request
     slots: torch.Tensor       # int64 [ntok] cache slot of every row, -1 for none
     positions: torch.Tensor   # int32 [ntok] position in its request, -1 for none
     free_count: torch.Tensor  # int32 [1] free pages left
+
+    def __setattr__(self, name, value):
+        old = self.__dict__.get(name)
+        object.__setattr__(self, name, value)
+        if old is not None:  # a buffer replaced after the first check
+            try:
+                self.__post_init__()
+            except ValueError:
+                object.__setattr__(self, name, old)
+                raise
 
     def __post_init__(self):
         n = self.length.numel()

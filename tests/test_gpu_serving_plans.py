@@ -41,3 +41,20 @@ def test_larger_buffers_serve_a_smaller_step():
         got.append((out, c.k.clone(), c.v.clone(), c.length.clone()))
     for a, b in zip(*got):
         assert torch.equal(a, b)
+
+
+def test_replaced_buffers_are_checked():
+    p = kv.plan_buffers(3, 8, "cuda")
+    for name, bad in (("length", torch.empty(4, dtype=torch.int32, device="cuda")), ("slots", i32([0] * 8)),
+                      ("kv_len", torch.empty(3, dtype=torch.int64, device="cuda")), ("kv_len", i32([0, 0])),
+                      ("q_start", i32([0] * 8)[::2]), ("free_count", i32([])),
+                      ("positions", torch.empty(8, dtype=torch.int32))):
+        old = getattr(p, name)
+        with pytest.raises(ValueError):
+            setattr(p, name, bad)
+        assert getattr(p, name) is old
+    p.length = i32([1, 2])  # fewer requests: the step may have two
+    table, free = i32([[-1] * 4] * 3), i32([0, 1, 2, 3])
+    with pytest.raises(ValueError):
+        kv.plan(table, i32([0, 0, 0]), i32([1, 1, 1]), free, i32([4]), 4, 8, out=p)
+    assert kv.plan(table[:2], i32([0, 0]), i32([1, 1]), free, i32([4]), 4, 8, out=p).kv_len.tolist() == [1, 1]
