@@ -15,7 +15,8 @@ namespace {
 constexpr int PLAN_THREADS = 1024;
 constexpr int SAT = 1 << 30;  // sums saturate here: past every size that is accepted
 
-CK_DEV int sat_add(int a, int b) { return min(a + b, SAT); }
+// two operands of 0 .. SAT: their sum fits an unsigned int, not an int
+CK_DEV int sat_add(int a, int b) { return (int)min((unsigned)a + (unsigned)b, (unsigned)SAT); }
 
 // Inclusive scan of three saturating sums over the CTA; the running carry is returned in place.
 struct Sum3 {

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from coherence_kernel_b200 import kv
+from tests import serving_ref as ref
 
 pytestmark = pytest.mark.gpu
 
@@ -58,3 +59,22 @@ def test_replaced_buffers_are_checked():
     with pytest.raises(ValueError):
         kv.plan(table, i32([0, 0, 0]), i32([1, 1, 1]), free, i32([4]), 4, 8, out=p)
     assert kv.plan(table[:2], i32([0, 0]), i32([1, 1]), free, i32([4]), 4, 8, out=p).kv_len.tolist() == [1, 1]
+
+
+@pytest.mark.parametrize("new", [[2 ** 31 - 1] * 2 + [1], [2 ** 31 - 1] * 4 + [1, 1], [1, 2 ** 30, 2 ** 30, 3], [2 ** 30] * 3,
+                                 [3, 2 ** 31 - 1, -2, 2 ** 30, -2 ** 31, 5] * 300])
+def test_row_counts_that_saturate(new):
+    """No request behind a sum of 2^30 rows or more is served, whatever the sum is."""
+    n = len(new)
+    table = [[3 * r % (3 * n), 3 * r + 1, -1, -1] for r in range(n)]
+    length = [5] * n
+    used = {p for row in table for p in row[:2]}
+    free = [p for p in range(3 * n) if p not in used]
+    free, count = free + [-9] * (3 * n - len(free)), len(free)
+    want = ref.plan(table, length, new, free, count, 4, 16, 3 * n)
+    t, f = i32(table), i32(free)
+    p = kv.plan(t, i32(length), i32(new), f, i32([count]), 4, 16)
+    got = (t.tolist(), f.tolist(), int(p.free_count), p.length.tolist(), p.kv_len.tolist(), p.q_start.tolist(),
+           p.slots.tolist(), p.positions.tolist())
+    for name, a, b in zip(("table", "free", "count", "length", "kv_len", "q_start", "slots", "positions"), got, want):
+        assert a == b, name
