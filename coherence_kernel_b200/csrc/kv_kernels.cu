@@ -133,7 +133,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_kv_plan(const KvPlanParams p) 
         }
     }
     const int back = n ? back_end[n - 1] : 0, need = n ? need_end[n - 1] : 0, rows = n ? row_end[n - 1] : 0;
-    const int top = count + back;
+    // at most n_blocks where the state is consistent; a count and lengths that are not may pass an int
+    const int top = (int)min((unsigned)count + (unsigned)back, 0x7fffffffu);
     // requests are served in order while their pages last; the rest of the requests that need pages
     // get none.  taken: the largest of the running sums that fits
     int taken = need;

@@ -78,3 +78,15 @@ def test_row_counts_that_saturate(new):
            p.slots.tolist(), p.positions.tolist())
     for name, a, b in zip(("table", "free", "count", "length", "kv_len", "q_start", "slots", "positions"), got, want):
         assert a == b, name
+
+
+def test_more_returned_pages_than_the_stack_holds():
+    """A count of all pages beside a request that returns three (no consistent state has that): nothing is written
+    outside the stack, whose size is the largest."""
+    n_blocks = 2 ** 31 - 1
+    free = torch.empty(n_blocks, dtype=torch.int32, device="cuda")
+    free[-4:] = i32([7, 8, 9, 10])
+    table = i32([[1, 2, 3, 4], [-1] * 4])
+    p = kv.plan(table, i32([3, 0]), i32([-3, 2]), free, i32([n_blocks]), 1, 4)
+    assert p.length.tolist() == [0, 2] and p.kv_len.tolist() == [0, 2] and int(p.free_count) == n_blocks - 2
+    assert free[-4:-2].tolist() == [7, 8] and p.positions.tolist() == [0, 1, -1, -1]
