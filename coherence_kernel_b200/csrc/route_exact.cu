@@ -20,7 +20,10 @@
 
 namespace ck {
 
+// tn-exp.  Halving never brings an infinity or a NaN below 1/2, so those take exp's limits and the loop ends after at
+// most 1025 halvings.
 CK_DEV double ref_exp(double x) {
+    if (isnan(x) || isinf(x)) return x < 0.0 ? 0.0 : x;
     int k = 0;
     for (;;) {
         const double ax = x < 0.0 ? 0.0 - x : x;
