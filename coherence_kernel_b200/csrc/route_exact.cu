@@ -391,20 +391,23 @@ CK_DEV void select_token(const double *sprob, const float *__restrict__ bias, in
             const int e = lane + 32 * r;
             if (e < ne && !(gon >> (e / gs) & 1)) v[r] = NEG;
         }
-        // dsv4-topk over the masked scores: the picks listed last-first
+        // dsv4-topk over the masked scores: the picks listed last-first.  A chosen expert gets the sentinel there and
+        // is passed over while others are above it; here it is passed over in any case, so that a token whose scores
+        // are not all numbers takes no expert twice (a tile of tokens has room for each once).
+        unsigned chosen = 0;
         for (int r = 0; r < k; ++r) {
             double b = -3.0e300;
             int bi = 1 << 30;
 #pragma unroll
             for (int rr = 0; rr < XS_MAXR; ++rr) {
                 const int e = lane + 32 * rr;
-                if (e < ne && v[rr] > b) { b = v[rr]; bi = e; }
+                if (e < ne && !(chosen >> rr & 1) && v[rr] > b) { b = v[rr]; bi = e; }
             }
             warp_argmax_d(b, bi);
             sel[k - 1 - r] = bi;
 #pragma unroll
             for (int rr = 0; rr < XS_MAXR; ++rr)
-                if (lane + 32 * rr == bi) v[rr] = NEG;
+                if (lane + 32 * rr == bi) chosen |= 1u << rr;
         }
         double s0 = 0.0;
         for (int i = 0; i < k; ++i) {

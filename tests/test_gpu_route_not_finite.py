@@ -41,3 +41,22 @@ def test_tokens_that_are_not_finite(spec, ntok):
     assert torch.isfinite(out[keep]).all()
     valid = (bids >= 0) & (bids < spec.n_experts)
     assert int(counts.sum()) == int(valid.sum())
+
+
+@pytest.mark.parametrize("spec", SPECS)
+@pytest.mark.parametrize("ntok", [1, 8, 300])
+def test_no_expert_is_taken_twice(spec, ntok):
+    """Two infinite activations whose weights have opposite signs for all experts but two: two scores are numbers."""
+    def router(w):
+        w = w.view(spec.n_experts, spec.hidden).clone()
+        w[:, 5], w[:, 900] = 0.25, -0.25
+        w[2, 900] = w[9, 900] = 0.25
+        return w
+    moe, x = layer(spec, ntok, router=router)
+    x[::2, 5] = x[::2, 900] = math.inf
+    out, ids, _, counts = moe(x)
+    moe.status(ntok)
+    for row in ids.tolist():
+        real = [e for e in row if 0 <= e < spec.n_experts]
+        assert len(set(real)) == len(real)
+    assert torch.isfinite(out[1::2]).all() and int(counts.max()) <= ntok
