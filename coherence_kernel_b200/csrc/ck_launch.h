@@ -169,10 +169,11 @@ int launch_gemm_dense(const GemmParams &p, cudaStream_t s);
 int launch_split_bf16x3(const float *w, uint16_t *out, uint32_t rows, uint32_t k, cudaStream_t s);
 
 // ---- serving around a paged KV cache.  Element types by GGUF number: 0 f32, 1 f16, 30 bf16, 8 Q8_0.
-// RMS norm with the residual's addition (norm_kernels.cu); strides in elements
+// RMS norm with the residual's addition (norm_kernels.cu); strides in elements.  live: NULL, or a row count on the
+// device; rows from it on take x as zero and leave res_out alone (not for Q8_0)
 int launch_rmsnorm_add(int x_type, const void *x, uint64_t x_stride, int res_type, const void *res, void *res_out,
                        uint64_t res_stride, const float *gain, int out_type, void *out, uint64_t out_stride,
-                       uint32_t ntok, uint32_t hidden, float eps, cudaStream_t s);
+                       uint32_t ntok, uint32_t hidden, float eps, cudaStream_t s, const int32_t *live = nullptr);
 // block tables and slot maps from request lengths, and the K/V write (kv_kernels.cu)
 constexpr uint32_t KV_PLAN_MAX_REQUESTS = 8192;  // three running sums and two lengths each in shared memory
 struct KvPlanParams {

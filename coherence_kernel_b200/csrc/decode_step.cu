@@ -62,8 +62,11 @@ __global__ void k_add_f32(float *__restrict__ h, const float *__restrict__ y, si
     const size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (i < n) h[i] = __fadd_rn(h[i], y[i]);
 }
-__global__ void k_add_bf16(float *__restrict__ h, const uint16_t *__restrict__ m, size_t n) {
+// live: NULL, or a row count: rows from it on (of H elements) are left alone
+__global__ void k_add_bf16(float *__restrict__ h, const uint16_t *__restrict__ m, size_t n,
+                           const int32_t *__restrict__ live, uint32_t H) {
     const size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i < n && live && (int64_t)(i / H) >= *live) return;
     if (i < n) h[i] = __fadd_rn(h[i], __uint_as_float((uint32_t)m[i] << 16));
 }
 
@@ -198,7 +201,7 @@ int ck_decode_step_run(ck_decode_step *s, float *h_dev, float *q_dev, float *k_d
     rc = ck_moe_layer_bf16(&s->cfg.moe, s->w.b, ntok, s->wg, s->wu, s->wd, s->sg, s->su, s->sd, s->router, s->bias,
                            s->w.ids, s->w.wts, s->w.counts, s->w.m, s->w.moe_ws, s->w.moe_ws_bytes, stream);
     if (rc) return rc;
-    k_add_bf16<<<eb, 256, 0, st>>>(h_dev, s->w.m, n);
+    k_add_bf16<<<eb, 256, 0, st>>>(h_dev, s->w.m, n, nullptr, s->cfg.hidden);
     return (int)cudaGetLastError();
 }
 
@@ -209,8 +212,8 @@ int ck_decode_step_capture(ck_decode_step *s, float *h_dev, float *q_dev, float 
 }
 
 static int check_step_kv(const ck_decode_step *s, const ck_step_kv *kv) {
-    if (!kv || !kv->cache || !kv->k_cache_dev || !kv->v_cache_dev || !kv->table_dev || !kv->kv_len_dev ||
-        !kv->q_start_dev || !kv->slots_dev || !kv->workspace_dev)
+    if (!kv || !kv->cache || !kv->k_cache_dev || !kv->v_cache_dev || !kv->q_start_dev || !kv->slots_dev ||
+        !kv->workspace_dev || (kv->nreq && (!kv->table_dev || !kv->kv_len_dev)))
         return CK_EARG;
     const ck_kv_config *c = kv->cache;
     if (c->n_kv_heads == 0 || kv->n_heads % c->n_kv_heads || (uint64_t)kv->n_heads * c->head_dim != s->cfg.hidden)
@@ -227,8 +230,11 @@ int ck_decode_step_run_kv(ck_decode_step *s, float *h_dev, float *q_dev, float *
     if (ntok > s->cfg.max_tokens) return CK_ESHAPE;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const uint32_t H = s->cfg.hidden, KV = kv->cache->n_kv_heads * kv->cache->head_dim;
-    rc = ck_rmsnorm_add(CK_F32, h_dev, H, CK_F32, nullptr, nullptr, 0, s->g_attn, CK_F32, s->w.a, H, ntok, H, s->cfg.eps,
-                        stream);
+    // Rows from q_start[nreq] on belong to no request, and the attention does not write them.  Their normed input is
+    // zero, so that zero is what its buffer holds there when the attention's output takes it over, and their h stays.
+    const int32_t *live = kv->q_start_dev + kv->nreq;
+    rc = ck::launch_rmsnorm_add(CK_F32, h_dev, H, CK_F32, nullptr, nullptr, 0, s->g_attn, CK_F32, s->w.a, H, ntok, H,
+                                s->cfg.eps, st, live);
     // matrices of one shape share a launch where the tensor-core matvec applies
     const uint8_t *wqkv[3] = {(const uint8_t *)s->wq, (const uint8_t *)s->wk, (const uint8_t *)s->wv};
     float *yqkv[3] = {q_dev, k_dev, v_dev};
@@ -249,14 +255,14 @@ int ck_decode_step_run_kv(ck_decode_step *s, float *h_dev, float *q_dev, float *
                                 stream);
     if (!rc) rc = ck::launch_q4k_matvec((const uint8_t *)s->wo, s->w.a, s->w.o, H, H, ntok, st);
     if (!rc)
-        rc = ck_rmsnorm_add(CK_F32, s->w.o, H, CK_F32, h_dev, h_dev, H, s->g_ffn, CK_BF16, s->w.b, H, ntok, H, s->cfg.eps,
-                            stream);
+        rc = ck::launch_rmsnorm_add(CK_F32, s->w.o, H, CK_F32, h_dev, h_dev, H, s->g_ffn, CK_BF16, s->w.b, H, ntok, H,
+                                    s->cfg.eps, st, live);
     if (!rc)
         rc = ck_moe_layer_bf16(&s->cfg.moe, s->w.b, ntok, s->wg, s->wu, s->wd, s->sg, s->su, s->sd, s->router, s->bias,
                                s->w.ids, s->w.wts, s->w.counts, s->w.m, s->w.moe_ws, s->w.moe_ws_bytes, stream);
     if (rc) return rc;
     const size_t n = (size_t)ntok * H;
-    k_add_bf16<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(h_dev, s->w.m, n);
+    k_add_bf16<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(h_dev, s->w.m, n, live, H);
     return (int)cudaGetLastError();
 }
 

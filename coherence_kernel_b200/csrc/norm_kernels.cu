@@ -33,6 +33,7 @@ struct NormArgs {
     uint32_t hidden;
     int x_type, res_type, out_type;
     float eps;
+    const int32_t *live;  // NULL, or a row count: rows from *live on take x as zero and leave res_out alone
 };
 
 CK_DEV void load_gain(const float *gain, uint32_t g, float (&v)[8]) {
@@ -63,12 +64,14 @@ __global__ void __launch_bounds__(VPT == 1 ? 1024 : VPT == 2 ? 512 : 256) k_rmsn
     grid_dep_wait();
     const uint32_t nv = p.hidden >> 3;
     const uint64_t row = blockIdx.x;
+    const bool pad = p.live && (int64_t)row >= *p.live;
     Raw8 rx[VPT], rr[VPT];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
         const uint32_t g = threadIdx.x + i * blockDim.x;
         if (g < nv) {
             rx[i] = load_raw8(p.x, row * p.x_stride + g * 8, p.x_type);
+            if (pad) rx[i].a = rx[i].b = make_uint4(0, 0, 0, 0);
             if (p.res) rr[i] = load_raw8(p.res, row * p.res_stride + g * 8, p.res_type);
         }
     }
@@ -84,7 +87,7 @@ __global__ void __launch_bounds__(VPT == 1 ? 1024 : VPT == 2 ? 512 : 256) k_rmsn
                 raw8_to_float(rr[i], p.res_type, r);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) s[i][j] += r[j];
-                if (p.res_out) store8(p.res_out, row * p.res_stride + g * 8, p.res_type, s[i]);
+                if (p.res_out && !pad) store8(p.res_out, row * p.res_stride + g * 8, p.res_type, s[i]);
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) acc += s[i][j] * s[i][j];
@@ -227,7 +230,8 @@ int launch(const NormArgs &a, uint32_t ntok, cudaStream_t s) {
 
 int launch_rmsnorm_add(int x_type, const void *x, uint64_t x_stride, int res_type, const void *res, void *res_out,
                        uint64_t res_stride, const float *gain, int out_type, void *out, uint64_t out_stride,
-                       uint32_t ntok, uint32_t hidden, float eps, cudaStream_t s) {
+                       uint32_t ntok, uint32_t hidden, float eps, cudaStream_t s, const int32_t *live) {
+    if (live && out_type == T_Q8_0) return CK_ERR_ARG;
     if (!float_type(x_type) || (res && !float_type(res_type)) || (out_type != T_Q8_0 && !float_type(out_type)))
         return CK_ERR_ARG;
     if (hidden == 0 || hidden % (out_type == T_Q8_0 ? 32 : 8) || hidden > 16384) return CK_ERR_SHAPE;
@@ -241,7 +245,7 @@ int launch_rmsnorm_add(int x_type, const void *x, uint64_t x_stride, int res_typ
         (out_type != T_Q8_0 && (out_stride < hidden || out_stride % 8)))
         return CK_ERR_ARG;
     const NormArgs a = {x, res, res_out, out, gain, x_stride, res_stride, out_stride, hidden, x_type, res_type,
-                        out_type, eps};
+                        out_type, eps, live};
     return launch(a, ntok, s);
 }
 

@@ -104,7 +104,8 @@ class DecodeStep:
                                                   _stream()), name)
 
     def run_kv(self, h, q, k, v, cache, plan, scale=None, window=0):
-        """The step over a paged cache: h [ntok, hidden] in place, the rows in the plan's order."""
+        """The step over a paged cache: h [ntok, hidden] in place, the rows in the plan's order.  Rows behind the
+        plan's last request are padding: their h stays as it is, and nothing of them enters the cache."""
         self._run_kv("ck_decode_step_run_kv", h, q, k, v, cache, plan, scale, window)
 
     def capture_kv(self, h, q, k, v, cache, plan, scale=None, window=0):

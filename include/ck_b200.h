@@ -426,7 +426,9 @@ int ck_paged_attention_status(const void *workspace_dev, void *stream);
  * The step's Wq and Wo are Q4_K [hidden x hidden], Wk and Wv [n_kv_heads * head_dim x hidden];
  * n_heads * head_dim == hidden.  No rotary embedding is applied, as in ck_decode_step_run.  q fp32
  * [ntok, hidden], k and v fp32 [ntok, n_kv_heads * head_dim] are outputs.  The rows are the plan's: a batch
- * mixes decodes and chunks freely within max_tokens.  The struct and *cache are read during the call only;
+ * mixes decodes and chunks freely within max_tokens.  Rows from q_start[nreq] on belong to no request (a batch padded
+ * to a captured size): their h is left as it is and nothing of them enters the cache, while q, k and v hold zeros there
+ * (NaNs where eps is 0).  Rows of requests that are not served attend over nothing and go through the rest of the step.  The struct and *cache are read during the call only;
  * a capture records the addresses in them, so that a plan that advances the same buffers before each
  * ck_decode_step_replay makes it the next step.  workspace: ck_paged_attention_workspace_bytes, zeroed first. */
 typedef struct {
