@@ -397,8 +397,12 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                             cp_wait<0>();
                             __syncwarp();  // a warp cleans the rows it copied
                             clean(tile + w * 32 * 128, item, 32, lane, 32, 32);
+                            // ordinary stores: the copies' own arrival does not order them
+                            fence_proxy_async_smem();
+                            mbar_arrive(&bar->full[st]);
+                        } else {
+                            hand_over(&bar->full[st]);
                         }
-                        hand_over(&bar->full[st]);
                         if (kv == 0 && c == it.c0) {  // the item's queries
                             ok = room(&bar->q_empty, (item & 1) ^ 1);
                             if (!ok) break;
