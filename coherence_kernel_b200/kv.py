@@ -156,7 +156,7 @@ def append(k, v, k_cache, v_cache, slots):
 class PagedAttention:
     """Attention of each request's new tokens over a paged cache (ck_paged_attention), with its
     workspace.  Calls that overlap in time (other streams, graphs replayed together) need an object
-    each."""
+    each, and the object has to be kept until its calls are done."""
 
     def __init__(self, n_heads: int, n_kv_heads: int, head_dim: int, max_tokens: int, max_requests: int,
                  device="cuda"):
@@ -166,6 +166,8 @@ class PagedAttention:
         if self.ws_bytes == 0:
             raise ValueError(f"unsupported heads: {n_heads} over {n_kv_heads} of {head_dim}")
         self.ws = torch.zeros(self.ws_bytes, dtype=torch.uint8, device=device)
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(self.ws.device).synchronize()  # zero before the first call on any stream
 
     def __call__(self, q, k_cache, v_cache, table, kv_len, q_start, scale: float | None = None, causal: bool = True,
                  window: int = 0, out=None, lse=None, return_lse: bool = False):
