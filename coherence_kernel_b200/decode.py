@@ -13,7 +13,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .kv import _config
+from .kv import _config, _window
 from .moe import MoeSpec
 from .ops import _dev, _ptr, _stream, q4k_nbytes
 
@@ -87,7 +87,7 @@ class DecodeStep:
             raise ValueError("the plan has more requests than the cache")
         kv = _lib.StepKv(ctypes.pointer(cfg), cache.k.data_ptr(), cache.v.data_ptr(), cache.table.data_ptr(),
                          cache.table.stride(0), plan.kv_len.data_ptr(), plan.q_start.data_ptr(),
-                         plan.slots.data_ptr(), cache.table.shape[1], nreq, at.n_heads, window,
+                         plan.slots.data_ptr(), cache.table.shape[1], nreq, at.n_heads, _window(window),
                          cfg.head_dim ** -0.5 if scale is None else scale, at.ws.data_ptr(), at.ws_bytes)
         return kv, ntok
 

@@ -125,6 +125,13 @@ def plan(table, length, new_tokens, free_blocks, free_count, block_tokens: int, 
     return o
 
 
+def _window(window):
+    """A window as the C argument: none (0) or a length; one past 32 bits bounds nothing, as any past the table's."""
+    if window < 0:
+        raise ValueError("window must not be negative")
+    return window if window < 1 << 31 else 0
+
+
 def _config(k_cache, v_cache):
     """ck_kv_config of cache tensors [n_blocks, block_tokens, n_kv_heads, head_dim] (any strides with
     contiguous heads, so a [n_blocks, n_kv_heads, block_tokens, head_dim] cache is passed permuted)."""
@@ -181,8 +188,6 @@ class PagedAttention:
         nreq, max_blocks = table.shape
         if ntok > self.max_tokens or nreq > self.max_requests:
             raise ValueError("more rows or requests than this object was made for")
-        if window < 0:
-            raise ValueError("window must not be negative")
         shape = (ntok, heads, dim)
         qs = _rows3(q, "q", shape, (k_cache.dtype, torch.float32), dev)
         if out is None:
@@ -200,7 +205,7 @@ class PagedAttention:
         _call("ck_paged_attention", dev, ctypes.byref(cfg), heads, TYPE_NUMBERS[q.dtype], q.data_ptr(), qs,
               k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), _table(table, dev), max_blocks,
               _ints(kv_len, "kv_len", nreq, dev), _ints(q_start, "q_start", nreq + 1, dev), nreq, ntok,
-              1.0 / math.sqrt(dim) if scale is None else scale, int(causal), window, out.data_ptr(), os_,
+              1.0 / math.sqrt(dim) if scale is None else scale, int(causal), _window(window), out.data_ptr(), os_,
               None if lse is None else lse.data_ptr(), self.ws.data_ptr(), self.ws_bytes)
         return (out, lse) if return_lse else out
 

@@ -63,3 +63,18 @@ def test_no_request_and_nobody_served():
     assert torch.equal(h, h0) and (cache.k == 0).all()
     a, cache = run(step, mk, 4, [[1000, 2, 0]], [8], [h0])  # 1000 rows do not fit
     assert (cache.k == 0).all() and not torch.equal(a, h0)
+
+
+def test_windows_of_the_step():
+    step, *_, mk, rng = make(4, 8, 6)
+    cache = mk()
+    plan = cache.plan(i32([3, 2, 1]), 6)
+    f = lambda w: torch.zeros((6, w), device="cuda")
+    with pytest.raises(ValueError):
+        step.run_kv(f(H), f(H), f(4 * D), f(4 * D), cache, plan, window=-1)
+    h0, hs = torch.from_numpy(rng.standard_normal((6, H)).astype("float32")).cuda(), []
+    for window in (0, 2 ** 32 + 1, 1):
+        h = h0.clone()
+        step.run_kv(h, f(H), f(4 * D), f(4 * D), cache, plan, window=window)
+        hs.append(h)
+    assert torch.equal(hs[0], hs[1]) and not torch.equal(hs[0], hs[2])

@@ -90,3 +90,17 @@ def test_more_returned_pages_than_the_stack_holds():
     p = kv.plan(table, i32([3, 0]), i32([-3, 2]), free, i32([n_blocks]), 1, 4)
     assert p.length.tolist() == [0, 2] and p.kv_len.tolist() == [0, 2] and int(p.free_count) == n_blocks - 2
     assert free[-4:-2].tolist() == [7, 8] and p.positions.tolist() == [0, 1, -1, -1]
+
+
+def test_windows_past_32_bits_and_negative_ones():
+    c = cache(n_heads=4)
+    g = torch.Generator().manual_seed(2)
+    q, k, v = (torch.randn(8, h, 64, generator=g).cuda() for h in (4, 2, 2))
+    p = c.plan(i32([8]), 8)
+    c.append(k, v, p)
+    want = c.attend(q, p)
+    for window in (2 ** 31, 2 ** 32 + 1, 10 ** 30):
+        assert torch.equal(c.attend(q, p, window=window), want)
+    assert not torch.equal(c.attend(q, p, window=1), want)
+    with pytest.raises(ValueError):
+        c.attend(q, p, window=-1)
