@@ -71,11 +71,7 @@ struct Sched {
         if (CHUNK ? rows < (int)p.row_split : rows >= (int)p.row_split) return 0;
         return (rows + TR - 1) / TR;
     }
-    // units of request r (all 32 lanes of a warp call this together, each with its own request)
-    static CK_DEV long long units(const AttnParams &p, int r) {
-        Req q;
-        return units(p, r, q);
-    }
+    // units of request r, which is returned in q (all 32 lanes of a warp call this together, each with its own request)
     static CK_DEV long long units(const AttnParams &p, int r, Req &q) {
         q = {0, 0, 0};
         if (r < (int)p.nreq) q = load_req(p, r);
