@@ -77,6 +77,7 @@ class DecodeStep:
         ntok = self._check(h, q, k, v)
         _lib.check(_lib.load().ck_decode_step_capture(self._h, _ptr(h), _ptr(q), _ptr(k), _ptr(v), ntok, _stream()),
                    "ck_decode_step_capture")
+        self._captured = (h, q, k, v)  # a replay writes them
 
     def _step_kv(self, cache, plan, scale, window):
         at, nreq, ntok = cache.attention, plan.kv_len.numel(), plan.slots.numel()
@@ -112,6 +113,7 @@ class DecodeStep:
         """Record run_kv over these buffers into a CUDA graph on the current (non-default) stream.  A plan
         into the same buffers (PagedKV.step_buffers) before each replay makes it the next step."""
         self._run_kv("ck_decode_step_capture_kv", h, q, k, v, cache, plan, scale, window)
+        self._captured = (h, q, k, v, cache, plan)  # a replay writes them
 
     def replay(self):
         _lib.check(_lib.load().ck_decode_step_replay(self._h, _stream()), "ck_decode_step_replay")

@@ -78,3 +78,23 @@ def test_windows_of_the_step():
         step.run_kv(h, f(H), f(4 * D), f(4 * D), cache, plan, window=window)
         hs.append(h)
     assert torch.equal(hs[0], hs[1]) and not torch.equal(hs[0], hs[2])
+
+
+def test_a_captured_step_holds_its_buffers():
+    """Buffers that only the captured step still refers to are not handed out again."""
+    step, *_, mk, rng = make(4, 8, 6)
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        cache = mk()
+        plan = cache.plan(i32([1, 1, 1]), 3, out=cache.step_buffers(3, 3))
+        h, q, k, v = (torch.zeros((3, w), device="cuda") for w in (H, H, 4 * D, 4 * D))
+        step.run_kv(h, q, k, v, cache, plan)
+        step.capture_kv(h, q, k, v, cache, plan)
+        step.replay()
+        sizes = [t.shape for t in (h, q, k, v, cache.attention.ws, cache.k, cache.v)]
+        s.synchronize()
+        del h, q, k, v, cache, plan
+        mine = [torch.full(z, 77.0, device="cuda", dtype=d) for z in sizes for d in (torch.float32, torch.uint8, torch.bfloat16)]
+        step.replay()
+    s.synchronize()
+    assert all((t == 77).all() for t in mine)
