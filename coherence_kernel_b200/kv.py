@@ -54,14 +54,17 @@ class Plan:
             _dev(t, name, dt, k)
             if t.device != self.length.device:
                 raise ValueError("the plan's buffers must be on one device")
+        # a plan of exactly n requests and ntok rows says so, so that a step into it checks one thing
+        ntok = self.slots.numel()
+        exact = self.kv_len.numel() == n and self.q_start.numel() == n + 1 and self.positions.numel() == ntok
+        object.__setattr__(self, "_fits", (n, ntok, self.length.device) if exact else None)
 
-    def cut(self, nreq: int, ntok: int) -> Plan:
+    def cut(self, nreq: int, ntok: int, device) -> Plan:
         """The plan of nreq requests and ntok rows in these buffers: itself, or views of their first elements."""
-        if (self.kv_len.numel() == nreq and self.slots.numel() == ntok and self.length.numel() == nreq
-                and self.q_start.numel() == nreq + 1 and self.positions.numel() == ntok):
+        if self._fits == (nreq, ntok, device):
             return self
-        if self.length.numel() < nreq or self.slots.numel() < ntok:
-            raise ValueError(f"out holds less than {nreq} requests and {ntok} rows")
+        if self.length.numel() < nreq or self.slots.numel() < ntok or self.length.device != device:
+            raise ValueError(f"out holds less than {nreq} requests and {ntok} rows, or is not on {device}")
         return Plan(self.length[:nreq], self.kv_len[:nreq], self.q_start[:nreq + 1], self.slots[:ntok],
                     self.positions[:ntok], self.free_count)
 
@@ -114,9 +117,7 @@ def plan(table, length, new_tokens, free_blocks, free_count, block_tokens: int, 
     if out is None:
         o = plan_buffers(nreq, ntok, dev)
     else:
-        if out.length.device != dev:
-            raise ValueError(f"out is not on {dev}")
-        o = out.cut(nreq, ntok)
+        o = out.cut(nreq, ntok, dev)
     _call("ck_kv_plan", dev, _ints(length, "length", nreq, dev), _ints(new_tokens, "new_tokens", nreq, dev), nreq,
           table.data_ptr(), stride, max_blocks, _ints(free_blocks, "free_blocks", 1, dev),
           _ints(free_count, "free_count", 1, dev), free_blocks.numel(), block_tokens, ntok, o.length.data_ptr(),
