@@ -128,7 +128,9 @@ int ck_swiglu_f32(const float *gate_dev, const float *up_dev, float *out_dev, ui
  * [ntok, nsel] (the reference's list order), counts int32 [ne], out bf16 [ntok, hidden].
  * Limits: ne <= 256, nsel <= 16, hidden % 64 == 0, inter % 64 == 0, ngroups <= 32.
  * tau: a token whose decision margin (smallest gap between a chosen and a rejected candidate's
- * fp32 score) is below tau is routed again in fp64 in the reference's own fold order. */
+ * fp32 score) is below tau is routed again in fp64 in the reference's own fold order.
+ * A token with a NaN or an infinity routes like any other, but where its scores are not numbers its ids may lie
+ * outside 0 .. ne - 1; such picks reach no expert and counts leaves them out.  Other tokens are not affected. */
 typedef struct {
     uint32_t hidden, inter, n_experts, n_shared, nsel, mode, ngroups, topk_groups;
     float wscale, tau;
@@ -344,9 +346,13 @@ void ck_ep_group_destroy(ck_ep_group *group);
  *   s = x[t] + res[t]  (s = x[t] where res is NULL);  res_out[t] = s in res_type (where not NULL; may be
  *   res itself);  out[t] = s / sqrt(mean(s^2) + eps) * gain.
  * x_type, res_type: CK_F32, CK_F16 or CK_BF16.  out_type: the same, or CK_Q8_0 -- GGUF blocks, row after
- * row: per 32 values d = f16(f32(max|v| / 127)) and codes round(v / d) in -127..127, from v in fp64.  Strides are in elements between rows (out_stride is not read for CK_Q8_0).
+ * row: per 32 values d = f16(f32(max|v| / 127)) and codes round(v / d) in -127..127, from v in fp64, halves to
+ * even.  (GGUF's own quantiser divides by the scale before its rounding to f16, and takes halves away from zero: the
+ * blocks mean the same, but single codes may differ by one from a file that other tools wrote.)  Strides are in
+ * elements between rows (out_stride is not read for CK_Q8_0).
  * A row that holds a NaN, or a block whose scale passes f16's range, has infinite scales: its values read
- * back as NaN.  hidden % 8 == 0 (32 for CK_Q8_0), hidden <= 16384, strides % 8 == 0 and >= hidden,
+ * back as NaN.  Beside CK_Q8_0, the sum of squares is fp32: a row's values have to stay below 1e17 (far beyond, the
+ * sum is infinite and the row zero).  hidden % 8 == 0 (32 for CK_Q8_0), hidden <= 16384, strides % 8 == 0 and >= hidden,
  * pointers 16-byte aligned (a CK_Q8_0 out: 2).  out must not overlap the inputs. */
 int ck_rmsnorm_add(int x_type, const void *x_dev, uint64_t x_stride, int res_type, const void *res_dev,
                    void *res_out_dev, uint64_t res_stride, const float *gain_dev, int out_type, void *out_dev,
@@ -403,8 +409,10 @@ int ck_kv_append(const ck_kv_config *cfg, int in_type, const void *k_dev, uint64
  * -infinity.  Rows q_start[nreq] .. are not touched; lengths beyond the table row or ntok are cut to
  * them; a table entry outside the cache is read as a page of zeros.  What a row does not see does not
  * reach it, infinities and NaNs among it (of what it sees: an infinite K element gives NaN in the f32 form).
- * io_type (q and out): the cache's type, with P rounded to it once before the second product, or CK_F32, which
- * keeps fp32 accuracy.  q_stride, out_stride: elements between rows, multiples of 8.  n_heads is a multiple
+ * io_type (q and out): the cache's type, with each p_j rounded to it once before the second product (off by half an ulp;
+ * an f16 one far below its row's largest by up to 2^-38 of that largest), or CK_F32, which keeps fp32's accuracy and
+ * range over either cache type.  Against 64 bits, on normal data, 16-bit outputs are off by 1.3 to 1.4 times what
+ * their own rounding alone would be.  q_stride, out_stride: elements between rows, multiples of 8.  n_heads is a multiple
  * of n_kv_heads, scale finite and > 0; ntok * n_heads < 2^30, max_blocks * block_tokens < 2^30.  ntok bounds the rows:
  * q_start[nreq] <= ntok.  workspace: ck_paged_attention_workspace_bytes (the same for every batch size), all zeros
  * before the first call with it and after a CK_ETIMEOUT (it counts the parts of work that spans CTAs, and every call
