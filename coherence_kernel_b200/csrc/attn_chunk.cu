@@ -22,9 +22,9 @@
 // round trip of O through registers.  P is rounded once to the cache's type, half an ulp of each weight:
 // against 64 bits the outputs are off by 1.4 times what their own rounding alone gives (2048 new tokens of 8192, bf16:
 // 0.0023 of their norm for 0.0017).  Scores, sums and O are fp32.  f16 weights are taken times 2^13 and rescaled at a
-// growth of 2, which keeps them below 65504: only those under 2^-27 of their row's largest fall among f16's
-// subnormals, where a weight is off by at most 2^-38 of the largest.  The maximum they refer to is rounded to a whole
-// number, so that neither the shift nor taking it back rounds anything (2048 new tokens of 8192: 249 us, as in bf16).
+// growth of 2.9, which keeps them below 2^15.9, within f16: only those under 2^-27 of their row's largest fall among f16's
+// subnormals, where a weight is off by at most 2^-38 of the largest.  The maximum they refer to is rounded down to a whole
+// number, so that neither the shift nor taking it back rounds anything (2048 new tokens of 8192: 247 us, as in bf16).
 //
 // Bounds per unit: the tensor core (4 x 128 x 128 x 128 multiply-adds, 2048 cycles), the exponentials (2 x 128 x 128 at 16
 // per cycle, 2048 cycles) and the tiles' way from L2 (64 KB at about 26 bytes per cycle, 2500 cycles) are close to
@@ -517,7 +517,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         // -------------------------------------------------------------------------------- softmax
         reg_inc<184>();
         // log2 growth of a row's maximum that makes O rescale, and the power of two that weights are raised by
-        constexpr float GROW = TYPE == T_F16 ? 2.0f : 8.0f, LIFT = TYPE == T_F16 ? 13.0f : 0.0f;
+        constexpr float GROW = TYPE == T_F16 ? 2.9f : 8.0f, LIFT = TYPE == T_F16 ? 13.0f : 0.0f;
         constexpr float DOWN = TYPE == T_F16 ? 0x1p-13f : 1.0f;
         const int t = wg, r = threadIdx.x & 127;  // tile of the item, row of the tile
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 lanes: lane number << 16
@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                                              __uint_as_float(s[2][31])),
                                         max3(mx[2], mx[3], __uint_as_float(s[3][31]))) *
                                   p.scale_log2;
-                const float whole_top = LIFT != 0.0f ? rintf(top) : top;
+                const float whole_top = LIFT != 0.0f ? floorf(top) : top;
                 if (c == it.c0) {
                     m = whole_top;
                 } else {
