@@ -29,8 +29,8 @@
 // Bounds per unit: the tensor core (4 x 128 x 128 x 128 multiply-adds, 2048 cycles), the exponentials (2 x 128 x 128 at 16
 // per cycle, 2048 cycles) and the tiles' way from L2 (64 KB at about 26 bytes per cycle, 2500 cycles) are close to
 // each other, and the chain scores - softmax - product of a half leaves gaps between them: about 4100 cycles.
-// 2048 new tokens of 8192, 32 heads over 8 of 128: 241 to 249 us, 980 TFLOP/s, 60% of the measured bf16 GEMM rate (tensor pipe 48%
-// active, special-function unit 48%).  Tried and slower: steps of 64 keys with their own score columns (271 us: an
+// 2048 new tokens of 8192, 32 heads over 8 of 128: 241 to 249 us, 980 TFLOP/s, 60% of the measured bf16 GEMM rate (tensor pipe 47%
+// active, special-function unit 47%).  Tried and slower: steps of 64 keys with their own score columns (271 us: an
 // N = 64 product of two shared-memory operands waits for shared memory), two threads per row (253), a
 // polynomial for a share of the exponentials (262 to 349, the share from 1/8 to 1/2).
 #include "attn_sched.cuh"
